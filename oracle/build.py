@@ -53,15 +53,15 @@ def ref_module_path():
 def build_ref(force=False):
     """Compile the reference's own C++ into oracle/_ref (needs /root/reference)."""
     out = ref_module_path()
-    if not os.path.isdir(REFERENCE_ROOT):
-        return out if os.path.exists(out) else None
-    import pybind11
-
-    os.makedirs(REF_DIR, exist_ok=True)
     src = os.path.join(HERE, "ref_wrap.cc")
     deps = [src,
             os.path.join(REFERENCE_ROOT, "det3d/ops/point_cloud/point_cloud_ops.h"),
             os.path.join(REFERENCE_ROOT, "det3d/ops/box2d_iou_rotated/src/box_iou_rotated_utils.h")]
+    if not all(os.path.exists(d) for d in deps):  # (an empty folder is no reference tree either)
+        return out if os.path.exists(out) else None
+    import pybind11
+
+    os.makedirs(REF_DIR, exist_ok=True)
     if force or _stale(out, deps):
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
                "-I", REFERENCE_ROOT, "-I", pybind11.get_include(),

@@ -44,6 +44,9 @@ FLAGS = [
     "-fPIC",
     "-ffp-contract=off",  # bit-exact f32 cell arithmetic / no surprise FMAs
     "-fhip-fp32-correctly-rounded-divide-sqrt",
+    # no packed f32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on gfx950.  The host
+    # pass of hipcc warns that it does not know the feature
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
     "-Wno-unused-function",
 ]
@@ -75,8 +78,9 @@ def _compile(src, force, hdr_m):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
-    if r.stderr.strip():
-        sys.stderr.write(r.stderr)
+    noise = [ln for ln in r.stderr.splitlines() if ln.strip() and "-packed-fp32-ops" not in ln and not ln.endswith("warning generated when compiling for host.") and not ln.endswith("warnings generated when compiling for host.")]
+    if noise:
+        sys.stderr.write("\n".join(noise) + "\n")
     return obj, True
 
 

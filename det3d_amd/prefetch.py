@@ -66,7 +66,7 @@ _RESERVED = {}  # device index -> stream created by reserve_stream
 
 
 def _new_stream(dev):
-    # small kernels: by default they may cut in front of the step's (D3D_PREFETCH_PRIORITY=0: equal priority)
+    # (the default priority, like every stream's: runtime "prefetch_priority")
     from . import runtime
 
     return torch.cuda.Stream(dev, priority=int(runtime.get("prefetch_priority")))
@@ -75,7 +75,7 @@ def _new_stream(dev):
 def reserve_stream(dev):
     """Create the geometry stream NOW and submit one trivial launch on it, so that the runtime binds it to a hardware
     queue before other libraries create their streams.  dist.init_dist calls this in front of init_process_group:
-    measured on MI355X (profiles/round4_multirank.txt), the same `Stream(priority=-1)` created AFTER the RCCL process
+    measured on MI355X (profiles/round4_multirank.txt), a geometry stream of high priority created AFTER the RCCL process
     group ran its ~75 small kernels per step at 40-90 us each instead of 5-15 us -- no longer cutting in front of the
     step's big kernels -- and the step waited 1.2 ms for its next batch's rulebooks (7.5 -> 8.8 ms)."""
     dev = torch.device(dev)

@@ -12,7 +12,8 @@ runs keep working), but the authoritative state is here and is settable from cod
                    data-gradient chain (sparse_stack / sparse_block / dense_stack; bit-identical results).  "sparse": not in
                    the dense RPN stack, whose two kernels are both MFMA-bound.  Default "all" (D3D_WGRAD_STREAM=0 -> "off").
   wgrad_priority   stream priority of that second stream (0; 1 = lower than the chain)        [D3D_WGRAD_PRIORITY]
-  prefetch_priority stream priority of the geometry stream (-1 = its small kernels cut in front) [D3D_PREFETCH_PRIORITY]
+  prefetch_priority stream priority of the geometry stream (0; -1 = its small kernels cut in front -- streams of different
+                   priorities have hung on MI355X, so every stream is at the default)             [D3D_PREFETCH_PRIORITY]
   pair_kernels     "off" | "measured" | "all": which f32 sparse launches take the pair-compacted kernel (spconv.PAIR_KERNELS)
   stack_executor   "python" | "c": the fused sparse stack's launches call by call from sparse_stack.py, or from one foreign call
                    per direction (csrc/d3d_stack.hip: same entry points, same order, bit-identical).  Default "python": the
@@ -38,7 +39,7 @@ _state = {
     "wgrad_stream": "off" if os.environ.get("D3D_WGRAD_STREAM", "1") == "0" else os.environ.get("D3D_WGRAD_STREAM_MODE", "all"),
     "wgrad_after_dgrad": os.environ.get("D3D_WGRAD_AFTER_DGRAD", "off"),
     "wgrad_priority": int(os.environ.get("D3D_WGRAD_PRIORITY", "0")),
-    "prefetch_priority": int(os.environ.get("D3D_PREFETCH_PRIORITY", "-1")),
+    "prefetch_priority": int(os.environ.get("D3D_PREFETCH_PRIORITY", "0")),
     "pair_kernels": os.environ.get("D3D_PAIR_KERNELS", "off"),
     "step_arena": os.environ.get("D3D_STEP_ARENA", "1") != "0",
     "geometry_ring": int(os.environ.get("D3D_GEOMETRY_RING", "3")),

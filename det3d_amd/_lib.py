@@ -73,6 +73,14 @@ SIGNATURES = {
     "d3d_pack_all": (i32, [vp, i32, vp]),
     "d3d_sparse_stack_forward": (i32, [vp, i32, i32, vp]),
     "d3d_sparse_stack_backward": (i32, [vp, i32, i32, vp, vp, vp]),
+    "d3d_act8_pitch": (i32, [i32]),
+    "d3d_act8_hold": (i32, [vp, i64, i64, i32, i32, i32, vp, vp, vp]),
+    "d3d_act8_restore": (i32, [vp, vp, i64, i32, i32, i32, vp, i64, vp]),
+    "d3d_act8_wgrad_workspace_bytes": (sz, [i64, i32, i32, i32, i32]),
+    "d3d_act8_wgrad": (i32, [vp, vp, i32, i64, i32, vp, i64, i32, i64, i32, vp, i64, i32, vp, vp, sz, vp]),
+    "d3d_row_join_fwd": (i32, [vp, vp]),
+    "d3d_row_join_ws_floats": (sz, [i64, i32, i32, i32]),
+    "d3d_row_join_bwd": (i32, [vp, vp, vp]),
     "d3d_conv2d_supported": (i32, [i32, i32, i32, i32]),
     "d3d_conv2d_supported_split3x3": (i32, [i32, i32]),
     "d3d_conv2d_stats_ws_floats": (sz, [i32, i32, i32, i32]),
@@ -166,6 +174,22 @@ class ChainLayer(ctypes.Structure):
 class DenseBnBackward(ctypes.Structure):
     """D3dDenseBnBackward of include/d3d.h"""
     _fields_ = [("x", vp), ("mean", vp), ("invstd", vp), ("gamma", vp), ("beta", vp), ("relu", i32)]
+
+
+class RowJoin(ctypes.Structure):
+    """D3dRowJoin of include/d3d.h"""
+    _fields_ = [("n", i64), ("c", i32), ("dtype", i32), ("fmt", i32), ("x", vp), ("x_stride", i64), ("f", vp), ("f_stride", i64),
+                ("gate", vp), ("gate_stride", i64), ("gate_cols", i32), ("gate_act", i32), ("scale", vp), ("alpha", f32),
+                ("post_kind", i32), ("post_eps", f32), ("post_weight", vp), ("post_bias", vp),
+                ("pre_kind", i32), ("pre_eps", f32), ("pre_weight", vp), ("pre_bias", vp), ("h", vp), ("z", vp),
+                ("x_codes", vp), ("x_scales", vp), ("f_codes", vp), ("f_scales", vp)]
+
+
+class RowJoinGrads(ctypes.Structure):
+    """D3dRowJoinGrads of include/d3d.h"""
+    _fields_ = [("dh", vp), ("dh_stride", i64), ("dz", vp), ("dz_stride", i64), ("dx", vp), ("df", vp), ("dgate", vp),
+                ("dscale", vp), ("dpost_weight", vp), ("dpost_bias", vp), ("dpre_weight", vp), ("dpre_bias", vp),
+                ("ws", vp), ("ws_floats", sz)]
 
 
 class AdamHyper(ctypes.Structure):

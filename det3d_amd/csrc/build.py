@@ -25,6 +25,8 @@ SOURCES = [
     "d3d_wgrad.hip",
     "d3d_stack.hip",
     "d3d_bn.hip",
+    "d3d_act8.hip",
+    "d3d_rownorm.hip",
     "d3d_conv2d.hip",
     "d3d_head.hip",
     "d3d_optim.hip",

@@ -1,0 +1,159 @@
+// Rows held in 8 bits (include/d3d.h, d3d_act8_*): the arithmetic that the hold / restore kernels, the row norms and the weight
+// gradient share, and the row vectors they move.
+//
+// 32 consecutive channels of a row form a group with one scale 2^s, stored as the biased exponent s + 127.  Powers of two make
+// x 2^-s and code 2^s exact, so which code a value gets depends on the value alone (no rounding in front of the rounding), and a
+// restored value has at most 8 significant bits: exact in bf16.
+#pragma once
+#include "d3d_common.h"
+
+#define A8_GROUP 32
+
+static inline int a8_pitch(int c) { return (c + A8_GROUP - 1) / A8_GROUP * A8_GROUP; }
+
+// biased exponent of a group's scale from the bits of its largest |x| (0xff: the group holds a NaN or an infinity).
+//   int8: rint(top 2^-s) <= 127  <=>  top 2^-s < 127.5 = 2^6 * 1.9921875 (the tie goes to the even 128): exponent - 6, one more
+//         from mantissa 0x7f0000 on;   e4m3: top 2^-s <= 448 = 2^8 * 1.75: exponent - 8, one more above mantissa 0x600000
+// The limits keep 2^-s and every code times 2^s normal and finite.
+template <int FMT> __device__ __forceinline__ uint32_t a8_scale_of(uint32_t top) {
+  if (top >= 0x7f800000u) return 0xffu;
+  int b = FMT == D3D_ACT8_INT8 ? (int)((top + 0x010000u) >> 23) - 6 : (int)((top + 0x1fffffu) >> 23) - 8;
+  constexpr int LO = FMT == D3D_ACT8_INT8 ? 127 - 120 : 127 - 110, HI = FMT == D3D_ACT8_INT8 ? 127 + 121 : 127 + 119;
+  return (uint32_t)(b < LO ? LO : (b > HI ? HI : b));
+}
+// 2^-s; 0 for a group of NaN (its codes are then zero, see a8_code4)
+__device__ __forceinline__ float a8_down(uint32_t b) { return b == 0xffu ? 0.f : __uint_as_float((254u - b) << 23); }
+// 2^s; infinity for 0xff, so that a zero code is restored as NaN
+__device__ __forceinline__ float a8_up(uint32_t b) { return __uint_as_float(b << 23); }
+
+// four codes in one word, value j in byte j
+template <int FMT> __device__ __forceinline__ uint32_t a8_code4(const float *v, float down) {
+  if (down == 0.f) return 0u;
+  if constexpr (FMT == D3D_ACT8_INT8) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float q = fminf(fmaxf(rintf(v[j] * down), -127.f), 127.f);
+      w |= ((uint32_t)(int)q & 0xffu) << (8 * j);
+    }
+    return w;
+  } else {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = fminf(fmaxf(v[j] * down, -448.f), 448.f);  // (the clip acts at the upper limit of s only)
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+  }
+}
+template <int FMT> __device__ __forceinline__ void a8_value4(uint32_t w, float up, float *v) {
+  if constexpr (FMT == D3D_ACT8_INT8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)((int)(w << (24 - 8 * j)) >> 24) * up;
+  } else {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = a[0] * up;
+    v[1] = a[1] * up;
+    v[2] = b[0] * up;
+    v[3] = b[1] * up;
+  }
+}
+
+typedef __attribute__((ext_vector_type(2))) float a8_f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 a8_bf16x2;
+__device__ __forceinline__ uint32_t a8_pack_bf16(float a, float b) {  // round to nearest even
+  const a8_f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, a8_bf16x2));
+}
+
+// E neighbouring values of a row in the feature type: one 16-byte access (E = 4 f32 / 8 bf16), or one value (E = 1) where the
+// row is not aligned to 16 bytes or its width is no multiple of E
+template <bool BF16, int E> struct A8Row {
+  static_assert(E == 1 || E == (BF16 ? 8 : 4), "one value or one 16-byte vector");
+  __device__ static __forceinline__ void load(const void *row, int64_t at, float *v) {
+    if constexpr (E == 1) {
+      if constexpr (BF16) v[0] = __uint_as_float((uint32_t)((const uint16_t *)row)[at] << 16);
+      else v[0] = ((const float *)row)[at];
+    } else if constexpr (BF16) {
+      const uint4 r = *(const uint4 *)((const uint16_t *)row + at);
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+      const float4 r = *(const float4 *)((const float *)row + at);
+      v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+    }
+  }
+  __device__ static __forceinline__ void store(void *row, int64_t at, const float *v) {
+    if constexpr (E == 1) {
+      if constexpr (BF16) ((uint16_t *)row)[at] = (uint16_t)(a8_pack_bf16(v[0], 0.f) & 0xffffu);
+      else ((float *)row)[at] = v[0];
+    } else if constexpr (BF16) {
+      uint4 r;
+      r.x = a8_pack_bf16(v[0], v[1]);
+      r.y = a8_pack_bf16(v[2], v[3]);
+      r.z = a8_pack_bf16(v[4], v[5]);
+      r.w = a8_pack_bf16(v[6], v[7]);
+      *(uint4 *)((uint16_t *)row + at) = r;
+    } else {
+      *(float4 *)((float *)row + at) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  }
+};
+
+// E values of a held row: LANES neighbouring lanes, each with E values, share a group (LANES * E = 32, or fewer where the
+// whole row is shorter)
+template <int FMT, int E, int LANES> struct A8Held {
+  // codes[at .. at + E) and, by the group's first lane, its scale; every lane of the group takes part
+  __device__ static __forceinline__ void store(uint8_t *codes, uint8_t *scales, int64_t row, int pitch, int at, bool inside,
+                                               const float *v) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const uint32_t u = __float_as_uint(v[j]) & 0x7fffffffu;
+      top = u > top ? u : top;
+    }
+#pragma unroll
+    for (int m = 1; m < LANES; m <<= 1) {
+      const uint32_t o = __shfl_xor(top, m, 64);
+      top = o > top ? o : top;
+    }
+    const uint32_t b = a8_scale_of<FMT>(top);
+    const float down = a8_down(b);
+    if (!inside) return;
+    uint8_t *c = codes + row * pitch + at;
+    if constexpr (E == 1) {
+      const float q[4] = {v[0], 0.f, 0.f, 0.f};
+      *c = (uint8_t)(a8_code4<FMT>(q, down) & 0xffu);
+    } else if constexpr (E == 4) {
+      *(uint32_t *)c = a8_code4<FMT>(v, down);
+    } else {
+      *(uint2 *)c = make_uint2(a8_code4<FMT>(v, down), a8_code4<FMT>(v + 4, down));
+    }
+    if ((at & (A8_GROUP - 1)) == 0) scales[row * (pitch / A8_GROUP) + at / A8_GROUP] = (uint8_t)b;
+  }
+  __device__ static __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t row, int pitch, int at,
+                                              float *v) {
+    const float up = a8_up(scales[row * (pitch / A8_GROUP) + at / A8_GROUP]);
+    const uint8_t *c = codes + row * pitch + at;
+    if constexpr (E == 1) {
+      float q[4];
+      a8_value4<FMT>(*c, up, q);
+      v[0] = q[0];
+    } else if constexpr (E == 4) {
+      a8_value4<FMT>(*(const uint32_t *)c, up, v);
+    } else {
+      const uint2 w = *(const uint2 *)c;
+      a8_value4<FMT>(w.x, up, v);
+      a8_value4<FMT>(w.y, up, v + 4);
+    }
+  }
+};
+
+// may rows of `elem_bytes` elements at p, `stride` elements apart and c wide, be moved as 16-byte vectors?
+static inline bool a8_vectors(const void *p, int64_t stride, int c, int elem_bytes) {
+  const int e = 16 / elem_bytes;
+  return p == nullptr || (((uintptr_t)p & 15) == 0 && stride % e == 0 && c % e == 0);
+}

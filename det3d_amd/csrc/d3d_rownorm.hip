@@ -1,0 +1,548 @@
+// Row norms and the join of a block (include/d3d.h, d3d_row_join_*):
+//
+//   forward   u = post(f);  h = x + alpha s act(g) u;  z = pre(h)            (f absent: h = x)
+//   backward  dH = dh + pre^T(dz);  dx = dH;  du = alpha s act(g) dH;  df = post^T(du);  dg = alpha s u act'(g) dH
+//             column sums: ds = alpha sum dH act(g) u, dw = sum dz hhat, db = sum dz, and the post norm's from du and fhat
+//   norm^T    with xhat = (x - mu) r and d = w dy:  r (d - mean(d) - xhat mean(d xhat));  rms has no mu and no mean(d)
+//
+// Bound by HBM: a few dozen f32 operations a value against 8 to 40 bytes.  So one pass: T lanes own a row and keep it in
+// registers (NV vectors of E values a lane) from the first load to the last store; the sums of a row go over the T lanes, by
+// shuffles up to a wave, through LDS beyond it.  The variance is a second sum over the registers, around the mean that the
+// first gave: no cancellation.  The backward pass recomputes u, h and their statistics from x and f (or from their 8-bit
+// codes) instead of reading saved ones.
+#include "d3d_act8.h"
+#include <string.h>
+
+
+template <int T, int NT, int N> __device__ __forceinline__ void row_sum(float *v, float (&lds)[2][N][NT / 64], int &slot) {
+#pragma unroll
+  for (int m = 1; m < (T < 64 ? T : 64); m <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m, 64);
+  if constexpr (T > 64) {
+    constexpr int W = T / 64;  // waves of a row
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) lds[slot][k][wave] = v[k];
+    }
+    d3d_lds_barrier();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) t += lds[slot][k][first + w];
+      v[k] = t;
+    }
+    slot ^= 1;
+  }
+}
+
+struct RjArgs {
+  D3dRowJoin a;
+  D3dRowJoinGrads g;
+  float inv_c;
+  int pitch;
+  float *part;     // backward: [blocks][sums][c] when the grid has more than one block, else null
+  int sums;
+};
+
+__device__ __forceinline__ void rj_act(int act, float g, float &a, float &da) {
+  if (act == D3D_GATE_NONE) {
+    a = g;
+    da = 1.f;
+    return;
+  }
+  const float p = 1.f / (1.f + expf(-g));
+  a = act == D3D_GATE_SIGMOID ? p : g * p;
+  da = act == D3D_GATE_SIGMOID ? p * (1.f - p) : p * (1.f + g * (1.f - p));
+}
+
+// T lanes own a row, NV vectors of E values each; RPB rows to a block of NT threads
+template <bool BF16_, int E_, int T_, int NV_> struct RjShape {
+  static constexpr bool BF16 = BF16_;
+  static constexpr int E = E_, T = T_, NV = NV_;
+  static constexpr int NT = T > 256 ? T : 256, RPB = NT / T, EPL = E * NV;
+};
+
+// (v - mu) and r of a row in place
+template <int T, int NT, int E, int NV>
+__device__ __forceinline__ float rj_normalise(int kind, float eps, float inv_c, int lane, int units, float *v,
+                                              float (&lds1)[2][1][NT / 64], int &slot) {
+  if (kind == D3D_NORM_LAYER) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < E * NV; ++j) s[0] += v[j];
+    row_sum<T, NT, 1>(s, lds1, slot);
+    const float mu = s[0] * inv_c;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = k * T + lane < units;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[k * E + j] = in ? v[k * E + j] - mu : 0.f;
+    }
+  }
+  float q[1] = {0.f};
+#pragma unroll
+  for (int j = 0; j < E * NV; ++j) q[0] = fmaf(v[j], v[j], q[0]);
+  row_sum<T, NT, 1>(q, lds1, slot);
+  return 1.f / sqrtf(fmaf(q[0], inv_c, eps));
+}
+
+template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fwd_kernel(RjArgs p) {
+  constexpr bool BF16 = S::BF16;
+  constexpr int E = S::E, T = S::T, NV = S::NV;
+  constexpr int GL = A8_GROUP / E < T ? A8_GROUP / E : T;
+  __shared__ float lds1[2][1][S::NT / 64];
+  int slot = 0;
+  const D3dRowJoin &a = p.a;
+  const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
+  const int c = a.c, units = c / E;
+  for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
+    const int64_t row = base + sub < a.n ? base + sub : a.n - 1;
+    const bool mine = base + sub < a.n;
+    float h[S::EPL];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int unit = k * T + lane;
+#pragma unroll
+      for (int j = 0; j < E; ++j) h[k * E + j] = 0.f;
+      if (unit < units) A8Row<BF16, E>::load(a.x, row * a.x_stride + unit * E, h + k * E);
+    }
+    if (a.x_codes) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+        A8Held<FMT, E, GL>::store(a.x_codes, a.x_scales, row, p.pitch, at, mine && at < p.pitch, h + k * E);
+      }
+    }
+    if (a.f) {
+      float f[S::EPL];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int unit = k * T + lane;
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[k * E + j] = 0.f;
+        if (unit < units) A8Row<BF16, E>::load(a.f, row * a.f_stride + unit * E, f + k * E);
+      }
+      if (a.f_codes) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int at = (k * T + lane) * E;
+          A8Held<FMT, E, GL>::store(a.f_codes, a.f_scales, row, p.pitch, at, mine && at < p.pitch, f + k * E);
+        }
+      }
+      float r = 1.f;
+      if (a.post_kind) r = rj_normalise<T, S::NT, E, NV>(a.post_kind, a.post_eps, p.inv_c, lane, units, f, lds1, slot);
+      float ag = 1.f, dag;
+      if (a.gate_cols == 1) {
+        A8Row<BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
+        rj_act(a.gate_act, ag, ag, dag);
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+        if (at >= c) continue;
+        float gt[E];
+        if (a.gate_cols > 1) A8Row<BF16, E>::load(a.gate, row * a.gate_stride + at, gt);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          float u = f[k * E + j] * r;
+          if (a.post_weight) u *= a.post_weight[at + j];
+          if (a.post_bias) u += a.post_bias[at + j];
+          float m = a.alpha * ag;
+          if (a.scale) m *= a.scale[at + j];
+          if (a.gate_cols > 1) {
+            float av;
+            rj_act(a.gate_act, gt[j], av, dag);
+            m *= av;
+          }
+          h[k * E + j] = fmaf(m, u, h[k * E + j]);
+        }
+        if (a.h && mine) A8Row<BF16, E>::store(a.h, row * (int64_t)c + at, h + k * E);
+      }
+    }
+    if (a.pre_kind) {
+      const float r = rj_normalise<T, S::NT, E, NV>(a.pre_kind, a.pre_eps, p.inv_c, lane, units, h, lds1, slot);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+        if (at >= c) continue;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          float z = h[k * E + j] * r;
+          if (a.pre_weight) z *= a.pre_weight[at + j];
+          if (a.pre_bias) z += a.pre_bias[at + j];
+          h[k * E + j] = z;
+        }
+        if (mine) A8Row<BF16, E>::store(a.z, row * (int64_t)c + at, h + k * E);
+      }
+    }
+  }
+}
+
+// the block's column sums: every lane's sums over the rows that it saw, added over the block's row groups in their order, into
+// the block's slab of the workspace (or, from a grid of one block, into the results)
+template <int E, int T, int NV, int NT>
+__device__ __forceinline__ void rj_columns(const float *acc, int c, float *lds, float *dst) {
+  constexpr int RPB = NT / T, EPL = E * NV;
+  const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int at = (k * T + lane) * E + j;
+        if (at < c) dst[at] = acc[k * E + j];
+      }
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < E; ++j) lds[sub * (T * EPL) + (k * T + lane) * E + j] = acc[k * E + j];
+    __syncthreads();
+    for (int at = threadIdx.x; at < c; at += NT) {
+      float t = 0.f;
+#pragma unroll
+      for (int s = 0; s < RPB; ++s) t += lds[s * (T * EPL) + at];
+      dst[at] = t;
+    }
+  }
+}
+
+// HELD: 0 rows as they are, 1 + format: codes
+template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_bwd_kernel(RjArgs p) {
+  constexpr bool BF16 = S::BF16;
+  constexpr int E = S::E, T = S::T, NV = S::NV;
+  constexpr int FMT = HELD == 2 ? D3D_ACT8_E4M3 : D3D_ACT8_INT8;
+  constexpr int GL = A8_GROUP / E < T ? A8_GROUP / E : T;
+  __shared__ float lds1[2][1][S::NT / 64], lds2[2][2][S::NT / 64], lds3[2][3][S::NT / 64];
+  __shared__ float cols[S::RPB > 1 ? S::NT * S::EPL : 1];
+  int slot1 = 0, slot2 = 0, slot3 = 0;
+  const D3dRowJoin &a = p.a;
+  const D3dRowJoinGrads &g = p.g;
+  const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
+  const int c = a.c, units = c / E;
+  const bool has_f = HELD ? a.f_codes != nullptr : a.f != nullptr;
+  float s_scale[S::EPL], s_pw[S::EPL], s_pb[S::EPL], s_qw[S::EPL], s_qb[S::EPL];
+#pragma unroll
+  for (int j = 0; j < S::EPL; ++j) s_scale[j] = s_pw[j] = s_pb[j] = s_qw[j] = s_qb[j] = 0.f;
+
+  for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
+    const int64_t row = base + sub < a.n ? base + sub : a.n - 1;
+    const bool mine = base + sub < a.n;
+    float h[S::EPL], f[S::EPL], m[S::EPL], dm[S::EPL];  // x, then h, then hhat | f, then fhat | factor of u | act'(g) alpha s
+    auto fetch = [&](const void *src, int64_t stride, const uint8_t *codes, const uint8_t *scales, float *v) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[k * E + j] = 0.f;
+        if (at < c) {
+          if constexpr (HELD) A8Held<FMT, E, GL>::load(codes, scales, row, p.pitch, at, v + k * E);
+          else A8Row<BF16, E>::load(src, row * stride + at, v + k * E);
+        }
+      }
+    };
+    fetch(a.x, a.x_stride, a.x_codes, a.x_scales, h);
+    float fr = 1.f, ag = 1.f, dag = 0.f;
+    if (has_f) {
+      fetch(a.f, a.f_stride, a.f_codes, a.f_scales, f);
+      if (a.post_kind) {
+        fr = rj_normalise<T, S::NT, E, NV>(a.post_kind, a.post_eps, p.inv_c, lane, units, f, lds1, slot1);
+#pragma unroll
+        for (int j = 0; j < S::EPL; ++j) f[j] *= fr;
+      }
+      if (a.gate_cols == 1) {
+        A8Row<BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
+        rj_act(a.gate_act, ag, ag, dag);
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+        float gt[E];
+        if (at < c && a.gate_cols > 1) A8Row<BF16, E>::load(a.gate, row * a.gate_stride + at, gt);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int q = k * E + j;
+          m[q] = dm[q] = 0.f;
+          if (at >= c) continue;
+          float av = ag, dv = dag;
+          if (a.gate_cols > 1) rj_act(a.gate_act, gt[j], av, dv);
+          m[q] = av;   // act(g)
+          dm[q] = dv;  // act'(g)
+          float u = f[q];
+          if (a.post_weight) u *= a.post_weight[at + j];
+          if (a.post_bias) u += a.post_bias[at + j];
+          const float s = a.scale ? a.alpha * a.scale[at + j] : a.alpha;
+          h[q] = fmaf(s * av, u, h[q]);
+        }
+      }
+    }
+    float d[S::EPL];  // dH
+    float hr = 1.f;
+    if (a.pre_kind) {
+      hr = rj_normalise<T, S::NT, E, NV>(a.pre_kind, a.pre_eps, p.inv_c, lane, units, h, lds1, slot1);
+      float s2[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+        float dz[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) dz[j] = 0.f;
+        if (at < c && g.dz) A8Row<BF16, E>::load(g.dz, row * g.dz_stride + at, dz);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int q = k * E + j;
+          h[q] *= hr;
+          d[q] = 0.f;
+          if (at >= c) continue;
+          d[q] = a.pre_weight ? dz[j] * a.pre_weight[at + j] : dz[j];
+          if (mine) {
+            s_qw[q] = fmaf(dz[j], h[q], s_qw[q]);
+            s_qb[q] += dz[j];
+          }
+          s2[0] = fmaf(d[q], h[q], s2[0]);
+          s2[1] += d[q];
+        }
+      }
+      row_sum<T, S::NT, 2>(s2, lds2, slot2);
+      const float m2 = s2[0] * p.inv_c, m1 = a.pre_kind == D3D_NORM_LAYER ? s2[1] * p.inv_c : 0.f;
+#pragma unroll
+      for (int j = 0; j < S::EPL; ++j) d[j] = hr * (d[j] - m1 - h[j] * m2);
+    } else {
+#pragma unroll
+      for (int j = 0; j < S::EPL; ++j) d[j] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int at = (k * T + lane) * E;
+      if (at >= c) continue;
+      if (g.dh) {
+        float dh[E];
+        A8Row<BF16, E>::load(g.dh, row * g.dh_stride + at, dh);
+#pragma unroll
+        for (int j = 0; j < E; ++j) d[k * E + j] += dh[j];
+      }
+      if (g.dx && mine) A8Row<BF16, E>::store(g.dx, row * (int64_t)c + at, d + k * E);
+    }
+    if (!has_f) continue;
+    float s3[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int at = (k * T + lane) * E;
+      if (at >= c) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) d[k * E + j] = 0.f;
+        continue;
+      }
+      float dg[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int q = k * E + j;
+        float u = f[q];
+        if (a.post_weight) u *= a.post_weight[at + j];
+        if (a.post_bias) u += a.post_bias[at + j];
+        const float s = a.scale ? a.alpha * a.scale[at + j] : a.alpha;
+        dg[j] = d[q] * s * u;
+        const float du = d[q] * s * m[q];
+        if (mine) {
+          s_scale[q] = fmaf(a.alpha * d[q] * m[q], u, s_scale[q]);
+          s_pw[q] = fmaf(du, f[q], s_pw[q]);
+          s_pb[q] += du;
+        }
+        s3[2] += dg[j];
+        dg[j] *= dm[q];
+        d[q] = a.post_weight ? du * a.post_weight[at + j] : du;
+        s3[0] = fmaf(d[q], f[q], s3[0]);
+        s3[1] += d[q];
+      }
+      if (g.dgate && a.gate_cols > 1 && mine) A8Row<BF16, E>::store(g.dgate, row * (int64_t)c + at, dg);
+    }
+    row_sum<T, S::NT, 3>(s3, lds3, slot3);
+    if (g.dgate && a.gate_cols == 1 && mine && lane == 0) {
+      const float v = s3[2] * dag;
+      A8Row<BF16, 1>::store(g.dgate, row, &v);
+    }
+    const float m2 = s3[0] * p.inv_c, m1 = a.post_kind == D3D_NORM_LAYER ? s3[1] * p.inv_c : 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int at = (k * T + lane) * E;
+      if (at >= c) continue;
+      if (a.post_kind) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) d[k * E + j] = fr * (d[k * E + j] - m1 - f[k * E + j] * m2);
+      }
+      if (g.df && mine) A8Row<BF16, E>::store(g.df, row * (int64_t)c + at, d + k * E);
+    }
+  }
+  float *const results[5] = {g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
+  const float *const accs[5] = {s_scale, s_pw, s_pb, s_qw, s_qb};
+  int at = 0;
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    if (!results[k]) continue;
+    rj_columns<E, T, NV, S::NT>(accs[k], c, cols, p.part ? p.part + ((int64_t)blockIdx.x * p.sums + at) * c : results[k]);
+    ++at;
+  }
+}
+
+__global__ void __launch_bounds__(256) row_join_fold_kernel(const float *__restrict__ part, int blocks, int sums, int c, D3dRowJoinGrads g) {
+  float *const all[5] = {g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < sums * c; i += gridDim.x * 256) {
+    float t = 0.f;
+    for (int b = 0; b < blocks; ++b) t += part[(int64_t)b * sums * c + i];
+    int left = i / c;
+    for (int k = 0; k < 5; ++k)
+      if (all[k] && left-- == 0) all[k][i % c] = t;
+  }
+}
+
+#define RJ_MAXC 8192
+static int rj_blocks_bwd(int64_t n, int rpb) {
+  const int64_t nb = (n + rpb - 1) / rpb;
+  return (int)(nb < 1 ? 1 : (nb > 512 ? 512 : nb));
+}
+
+static int rj_check(const D3dRowJoin *a, bool backward, const char *who) {
+  D3D_REQUIRE(a, "%s: null pointer", who);
+  D3D_REQUIRE(a->dtype == D3D_F32 || a->dtype == D3D_BF16, "%s: dtype %d", who, a->dtype);
+  D3D_REQUIRE(a->fmt == D3D_ACT8_INT8 || a->fmt == D3D_ACT8_E4M3, "%s: format %d", who, a->fmt);
+  D3D_REQUIRE(a->n >= 1 && a->n < ((int64_t)1 << 40) && a->c >= 1 && a->c <= RJ_MAXC, "%s: %lld rows of %d channels (1 to %d)", who,
+              (long long)a->n, a->c, RJ_MAXC);
+  const bool held = a->x_codes != nullptr;
+  D3D_REQUIRE(a->x || (backward && held), "%s: no rows", who);
+  D3D_REQUIRE(!a->x || a->x_stride >= a->c, "%s: x rows %lld elements apart", who, (long long)a->x_stride);
+  D3D_REQUIRE(!a->f || a->f_stride >= a->c, "%s: f rows %lld elements apart", who, (long long)a->f_stride);
+  D3D_REQUIRE(held == (a->x_scales != nullptr) && (a->f_codes != nullptr) == (a->f_scales != nullptr), "%s: codes without scales", who);
+  const bool has_f = a->f || a->f_codes;
+  D3D_REQUIRE(!has_f || backward || held == (a->f_codes != nullptr), "%s: x and f are held together", who);
+  D3D_REQUIRE(!backward || !held || !has_f || a->f_codes, "%s: x is held in 8 bits, f is not", who);
+  D3D_REQUIRE(has_f || !a->f_codes, "%s: codes of f without f", who);
+  D3D_REQUIRE(a->post_kind >= 0 && a->post_kind <= 2 && a->pre_kind >= 0 && a->pre_kind <= 2, "%s: norm kinds %d, %d", who, a->post_kind, a->pre_kind);
+  D3D_REQUIRE(a->post_eps >= 0.f && a->pre_eps >= 0.f, "%s: negative eps", who);
+  D3D_REQUIRE(has_f || (a->pre_kind && !a->post_kind && !a->gate && !a->scale), "%s: without f there is the pre norm alone", who);
+  D3D_REQUIRE(a->gate ? (a->gate_cols == 1 || a->gate_cols == a->c) && a->gate_stride >= a->gate_cols : a->gate_cols == 0, "%s: gate of %d columns", who, a->gate_cols);
+  D3D_REQUIRE(a->gate_act >= D3D_GATE_NONE && a->gate_act <= D3D_GATE_SILU, "%s: gate_act %d", who, a->gate_act);
+  D3D_REQUIRE((((uintptr_t)a->x_codes | (uintptr_t)a->f_codes) & 15) == 0, "%s: codes are not aligned to 16 bytes", who);
+  return D3D_OK;
+}
+// may the rows be moved as 16-byte vectors?  (the float32 vectors over the channels are read value by value)
+static bool rj_vectors(const D3dRowJoin *a, const D3dRowJoinGrads *g) {
+  const int eb = a->dtype == D3D_BF16 ? 2 : 4;
+  bool v = a8_vectors(a->x, a->x_stride, a->c, eb) && a8_vectors(a->f, a->f_stride, a->c, eb) && a8_vectors(a->h, a->c, a->c, eb) &&
+           a8_vectors(a->z, a->c, a->c, eb) && a->c % (16 / eb) == 0;
+  if (a->gate_cols > 1) v = v && a8_vectors(a->gate, a->gate_stride, a->c, eb);
+  if (g) {
+    v = v && a8_vectors(g->dh, g->dh_stride, a->c, eb) && a8_vectors(g->dz, g->dz_stride, a->c, eb) &&
+        a8_vectors(g->dx, a->c, a->c, eb) && a8_vectors(g->df, a->c, a->c, eb);
+    if (a->gate_cols > 1) v = v && a8_vectors(g->dgate, a->c, a->c, eb);
+  }
+  return v;
+}
+
+// The shape of the launch by the number of units (16-byte vectors, or values of unaligned rows) in a row: the fewest lanes that
+// hold it with at most 8 values a lane.  go(RjShape) launches.
+template <bool BF16, class Go> static int rj_pick(int c, bool vec, Go &&go) {
+  constexpr int E = BF16 ? 8 : 4;
+  if (vec) {
+    const int units = c / E;
+    if (units <= 8) return go(RjShape<BF16, E, 8, 1>{});
+    if (units <= 16) return go(RjShape<BF16, E, 16, 1>{});
+    if (units <= 32) return go(RjShape<BF16, E, 32, 1>{});
+    if (units <= 64) return go(RjShape<BF16, E, 64, 1>{});
+    if (units <= 128) return go(RjShape<BF16, E, 128, 1>{});
+    if (units <= 256) return go(RjShape<BF16, E, 256, 1>{});
+    if (units <= 512) return go(RjShape<BF16, E, 512, 1>{});
+    if (units <= 1024) return go(RjShape<BF16, E, BF16 ? 1024 : 512, BF16 ? 1 : 2>{});
+    return go(RjShape<BF16, E, 1024, BF16 ? 1 : 2>{});
+  }
+  if (c <= 32) return go(RjShape<BF16, 1, 32, 1>{});
+  if (c <= 64) return go(RjShape<BF16, 1, 64, 1>{});
+  if (c <= 256) return go(RjShape<BF16, 1, 64, 4>{});
+  if (c <= 1024) return go(RjShape<BF16, 1, 256, 4>{});
+  return go(RjShape<BF16, 1, 1024, 8>{});
+}
+template <class Go> static int rj_for(const D3dRowJoin *a, bool vec, Go &&go) {
+  return a->dtype == D3D_BF16 ? rj_pick<true>(a->c, vec, go) : rj_pick<false>(a->c, vec, go);
+}
+
+extern "C" int d3d_row_join_fwd(const D3dRowJoin *a, d3d_stream_t stream_) {
+  hipStream_t stream = (hipStream_t)stream_;
+  int rc = rj_check(a, false, "d3d_row_join_fwd");
+  if (rc) return rc;
+  D3D_REQUIRE((a->h || !a->f) && (a->z || !a->pre_kind), "d3d_row_join_fwd: null output");
+  const bool vec = rj_vectors(a, nullptr);
+  RjArgs p;
+  memset(&p, 0, sizeof(p));
+  p.a = *a;
+  p.inv_c = 1.f / (float)a->c;
+  p.pitch = a8_pitch(a->c);
+  rj_for(a, vec, [&](auto shape) {
+    using S = decltype(shape);
+    const int64_t nb = (a->n + S::RPB - 1) / S::RPB;
+    const dim3 grid((unsigned)(nb > 65536 ? 65536 : nb));
+    if (a->fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((row_join_fwd_kernel<S, D3D_ACT8_INT8>), grid, dim3(S::NT), 0, stream, p);
+    else hipLaunchKernelGGL((row_join_fwd_kernel<S, D3D_ACT8_E4M3>), grid, dim3(S::NT), 0, stream, p);
+    return D3D_OK;
+  });
+  D3D_LAUNCH_TRY("row_join_fwd_kernel");
+  return D3D_OK;
+}
+
+// workspace of the column sums: an upper bound over the row layouts (rows per block), which depend on alignment too
+extern "C" size_t d3d_row_join_ws_floats(int64_t n, int c, int dtype, int sums) {
+  if (n < 1 || c < 1 || c > RJ_MAXC || sums < 1 || sums > 5 || (dtype != D3D_F32 && dtype != D3D_BF16)) return 0;
+  return (size_t)rj_blocks_bwd(n, 1) * (size_t)sums * (size_t)c;
+}
+
+extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d3d_stream_t stream_) {
+  hipStream_t stream = (hipStream_t)stream_;
+  int rc = rj_check(a, true, "d3d_row_join_bwd");
+  if (rc) return rc;
+  D3D_REQUIRE(g, "d3d_row_join_bwd: null pointer");
+  const bool has_f = a->f || a->f_codes;
+  D3D_REQUIRE(!g->dh || g->dh_stride >= a->c, "d3d_row_join_bwd: dh rows %lld elements apart", (long long)g->dh_stride);
+  D3D_REQUIRE(!g->dz || g->dz_stride >= a->c, "d3d_row_join_bwd: dz rows %lld elements apart", (long long)g->dz_stride);
+  D3D_REQUIRE(!g->dz || a->pre_kind, "d3d_row_join_bwd: dz without a pre norm");
+  D3D_REQUIRE(has_f || (!g->dh && !g->df), "d3d_row_join_bwd: dh / df without f");
+  D3D_REQUIRE(!g->dgate || a->gate, "d3d_row_join_bwd: dgate without a gate");
+  D3D_REQUIRE((!g->dscale || a->scale) && (!g->dpost_weight || a->post_weight) && (!g->dpost_bias || a->post_bias) &&
+                  (!g->dpre_weight || a->pre_weight) && (!g->dpre_bias || a->pre_bias),
+              "d3d_row_join_bwd: the gradient of an absent vector");
+  const int sums = !!g->dscale + !!g->dpost_weight + !!g->dpost_bias + !!g->dpre_weight + !!g->dpre_bias;
+  const bool vec = rj_vectors(a, g);
+  RjArgs p;
+  memset(&p, 0, sizeof(p));
+  p.a = *a;
+  p.g = *g;
+  p.inv_c = 1.f / (float)a->c;
+  p.pitch = a8_pitch(a->c);
+  p.sums = sums;
+  const int held = a->x_codes ? 1 + a->fmt : 0;
+  int blocks = 0;
+  rc = rj_for(a, vec, [&](auto shape) {
+    using S = decltype(shape);
+    blocks = rj_blocks_bwd(a->n, S::RPB);
+    if (sums && blocks > 1) {
+      const size_t need = (size_t)blocks * sums * a->c;
+      if (!g->ws || g->ws_floats < need)
+        return d3d_set_error(D3D_ECAPACITY, "d3d_row_join_bwd: workspace of %zu floats, %zu needed", (size_t)g->ws_floats, need);
+      p.part = g->ws;
+    }
+    const dim3 grid((unsigned)blocks), block(S::NT);
+    if (held == 0) hipLaunchKernelGGL((row_join_bwd_kernel<S, 0>), grid, block, 0, stream, p);
+    else if (held == 1) hipLaunchKernelGGL((row_join_bwd_kernel<S, 1>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((row_join_bwd_kernel<S, 2>), grid, block, 0, stream, p);
+    return D3D_OK;
+  });
+  if (rc) return rc;
+  D3D_LAUNCH_TRY("row_join_bwd_kernel");
+  if (p.part) {
+    const int nb = (sums * a->c + 255) / 256;
+    hipLaunchKernelGGL(row_join_fold_kernel, dim3(nb), dim3(256), 0, stream, p.part, blocks, sums, a->c, *g);
+    D3D_LAUNCH_TRY("row_join_fold_kernel");
+  }
+  return D3D_OK;
+}

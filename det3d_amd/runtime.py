@@ -1,4 +1,5 @@
-"""Run-time configuration of the hot path: the switches that change HOW a step is scheduled (never what it computes).
+"""Run-time configuration of the hot path: the switches that change HOW a step is scheduled (and, `activations` alone, what it
+computes).
 
 behaviour that changes a result's timing belongs in the configuration, not in
 environment variables read at import.  The variables still exist as DEFAULTS (so that `tools/gpu_job.sh env:VAR=..` A/B
@@ -20,6 +21,11 @@ runs keep working), but the authoritative state is here and is settable from cod
                    executor changes neither the step time nor the process's CPU time per step (15.1 vs 15.3 ms, bf16 and
                    f32 alike, profiles/round6_stack_executor.txt) -- it is not the interpreter that bounds the host
                    [D3D_STACK_EXECUTOR]
+  activations      "full" | "int8" | "e4m3": what the sparse convolutions, the BatchNorm sweeps behind them and RowNorm keep for the
+                   backward pass -- their rows as they are, or in 8 bits (act8.py).  The one switch here that changes what a
+                   step computes: gradients are taken at the restored rows.  In 8 bits the layers run one by one (the fused
+                   sparse nodes keep full rows) and TrainStep leaves its step arena aside, so that rows are freed as the
+                   forward pass goes on; default "full"                                               [D3D_ACTIVATIONS]
   step_arena       TrainStep's default for its step arena (arena.py)
   geometry_ring    slots of GeometryPrefetcher's arena ring (0 = caching allocator)
 
@@ -34,6 +40,7 @@ _VALID = {
     "pair_kernels": ("off", "measured", "all"),
     "geometry_gate": ("off", "sparse_fwd"),
     "stack_executor": ("c", "python"),
+    "activations": ("full", "int8", "e4m3"),
 }
 _state = {
     "wgrad_stream": "off" if os.environ.get("D3D_WGRAD_STREAM", "1") == "0" else os.environ.get("D3D_WGRAD_STREAM_MODE", "all"),
@@ -45,6 +52,7 @@ _state = {
     "geometry_ring": int(os.environ.get("D3D_GEOMETRY_RING", "3")),
     "geometry_gate": os.environ.get("D3D_GEOMETRY_GATE", "off"),
     "stack_executor": os.environ.get("D3D_STACK_EXECUTOR", "python"),
+    "activations": os.environ.get("D3D_ACTIVATIONS", "full"),
 }
 
 
@@ -54,6 +62,12 @@ def get(name):
 
 def describe():
     return dict(_state)
+
+
+def held_format():
+    """the 8-bit format that layers keep their rows in between the two passes, None where they keep them as they are"""
+    a = _state["activations"]
+    return None if a == "full" else a
 
 
 def wgrad_side(kind):

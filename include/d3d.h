@@ -467,6 +467,84 @@ int d3d_channel_affine_bwd(const void *x, const void *dy, int n, int c, int dtyp
                            const float *coef_1, void *dx, d3d_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Rows held in 8 bits between the forward and the backward pass (csrc/d3d_act8.hip).  The reference keeps every activation
+ * of a training step in full (autograd's saved tensors behind det3d/models/backbones/scn.py:106-157); a held row takes 1.03
+ * bytes a value.  32 consecutive channels of a row form a group with one scale 2^s, stored as the biased exponent s + 127:
+ *   D3D_ACT8_INT8  s the smallest with rint(max|x| 2^-s) <= 127, s in [-120, 121]; codes int8 rint(x 2^-s), clipped to +-127
+ *   D3D_ACT8_E4M3  s the smallest with max|x| 2^-s <= 448, s in [-110, 119];       codes OCP e4m3 of x 2^-s, clipped to +-448
+ * A group with a NaN or an infinity has scale byte 255 and is restored as NaN.  Restored values are exact in bf16.
+ *   x      dev [n, c] dtype, rows x_stride (>= c) elements apart
+ *   codes  dev [n, d3d_act8_pitch(c)] bytes (c rounded up to 32; zero behind channel c), 16-byte aligned;
+ *   scales dev [n, d3d_act8_pitch(c) / 32] bytes
+ * d3d_act8_wgrad: dw[k][ci][co] = sum_o x[nbr[k * cap + o]][ci] dy[o][co] over the held rows [n_in, cin] and dy [n_out, cout]
+ *   dtype (rows dy_stride apart), dw dev [kvol, cin, cout] f32, overwritten; entries of nbr outside [0, n_in) add nothing;
+ *   nbr NULL (kvol 1, n_in == n_out): dw = x^T dy.  Products exact to f32, f32 sums in a fixed order.  workspace:
+ *   d3d_act8_wgrad_workspace_bytes (may be 0), need not be zeroed. */
+#define D3D_ACT8_INT8 0
+#define D3D_ACT8_E4M3 1
+int d3d_act8_pitch(int c);
+int d3d_act8_hold(const void *x, int64_t x_stride, int64_t n, int c, int dtype, int fmt, uint8_t *codes, uint8_t *scales,
+                  d3d_stream_t stream);
+int d3d_act8_restore(const uint8_t *codes, const uint8_t *scales, int64_t n, int c, int fmt, int dtype, void *out,
+                     int64_t out_stride, d3d_stream_t stream);
+size_t d3d_act8_wgrad_workspace_bytes(int64_t n_out, int kvol, int cin, int cout, int dtype);
+int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int fmt, int64_t n_in, int cin, const void *dy,
+                   int64_t dy_stride, int dtype, int64_t n_out, int cout, const int32_t *nbr, int64_t cap, int kvol, float *dw,
+                   void *workspace, size_t workspace_bytes, d3d_stream_t stream);
+
+/* Norms of rows over their channels and the join of a residual block between them (csrc/d3d_rownorm.hip): the row-wise
+ * counterpart of the BatchNorm sweeps above, for blocks of the shape det3d/models/backbones/scn.py:76-87 (norm, identity add).
+ *   u = post(f);  h = x + alpha * scale * act(gate) * u;  z = pre(h)
+ *   norm kinds: D3D_NORM_NONE; RMS  v * r * w + b, r = 1 / sqrt(mean v^2 + eps); LAYER  (v - mean) * r * w + b
+ * n >= 1 rows of 1 <= c <= 8192 channels, dtype; x, f, gate, dh, dz: rows *_stride elements apart; h, z, dx, df, dgate
+ * contiguous.  f NULL: z = pre(x), h unused.  gate_cols 0 (no gate) | 1 (one value a row) | c.  scale, weights, biases: dev [c]
+ * f32 or NULL.  fwd with x_codes / x_scales (and f_codes / f_scales with f) writes x and f in 8 bits of format fmt in the
+ * same pass; bwd with them reads the codes in place of x and f (which may then be NULL) and gives the gradients at the restored
+ * rows.  z may be NULL without a pre norm.
+ * bwd: dh, dz dev [n, c] dtype, either NULL = zero; every result may be NULL; dgate [n, gate_cols] dtype; dscale, dpost_*,
+ * dpre_* dev [c] f32, overwritten; ws: d3d_row_join_ws_floats(n, c, dtype, number of [c] results asked for) floats. */
+#define D3D_NORM_NONE 0
+#define D3D_NORM_RMS 1
+#define D3D_NORM_LAYER 2
+#define D3D_GATE_NONE 0
+#define D3D_GATE_SIGMOID 1
+#define D3D_GATE_SILU 2
+typedef struct D3dRowJoin {
+  int64_t n;
+  int c, dtype, fmt;
+  const void *x;
+  int64_t x_stride;
+  const void *f;
+  int64_t f_stride;
+  const void *gate;
+  int64_t gate_stride;
+  int gate_cols, gate_act;
+  const float *scale;
+  float alpha;
+  int post_kind;
+  float post_eps;
+  const float *post_weight, *post_bias;
+  int pre_kind;
+  float pre_eps;
+  const float *pre_weight, *pre_bias;
+  void *h, *z;
+  uint8_t *x_codes, *x_scales, *f_codes, *f_scales;
+} D3dRowJoin;
+typedef struct D3dRowJoinGrads {
+  const void *dh;
+  int64_t dh_stride;
+  const void *dz;
+  int64_t dz_stride;
+  void *dx, *df, *dgate;
+  float *dscale, *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+  float *ws;
+  size_t ws_floats;
+} D3dRowJoinGrads;
+int d3d_row_join_fwd(const D3dRowJoin *args, d3d_stream_t stream);
+size_t d3d_row_join_ws_floats(int64_t n, int c, int dtype, int sums);
+int d3d_row_join_bwd(const D3dRowJoin *args, const D3dRowJoinGrads *grads, d3d_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Dense 2D convolution on channels-last maps: the RPN's conv layers (det3d/models/necks/rpn.py:70-159, nn.Conv2d
  * 3x3 stride 1/2 and the 1x1 / 2x2 deblock convs, bias-free; the reference runs them on cuDNN).  Implicit GEMM on
  * MFMA, both operands through LDS-DMA, f32 accumulation.

@@ -1,0 +1,114 @@
+"""Argument checks of the operators on held rows and row norms (d3d_act8_*, d3d_row_join_*): they run before any HIP call, so no GPU
+is needed; what the Python layer refuses without one; workspace sizes."""
+import ctypes
+
+import pytest
+import torch
+
+
+def err(L):
+    return L.d3d_last_error()
+
+
+def test_pitch_and_workspaces(hip_lib):
+    L = hip_lib
+    assert [L.d3d_act8_pitch(c) for c in (1, 31, 32, 33, 64, 4096)] == [32, 32, 32, 64, 64, 4096]
+    assert L.d3d_act8_pitch(0) == 0 and L.d3d_act8_pitch(-3) == 0
+    from det3d_amd import act8
+
+    assert all(act8.pitch(c) == L.d3d_act8_pitch(c) for c in range(1, 300))
+    assert L.d3d_act8_wgrad_workspace_bytes(0, 27, 64, 64, 0) == 0 and L.d3d_act8_wgrad_workspace_bytes(100, 27, 64, 64, 9) == 0
+    big = L.d3d_act8_wgrad_workspace_bytes(100000, 27, 64, 64, 0)
+    assert big % (27 * 64 * 64 * 4) == 0 and big < 1 << 30
+    assert L.d3d_row_join_ws_floats(100, 64, 0, 5) >= 5 * 64
+    for bad in ((0, 64, 0, 5), (100, 0, 0, 5), (100, 8193, 0, 5), (100, 64, 2, 5), (100, 64, 0, 0), (100, 64, 0, 6)):
+        assert L.d3d_row_join_ws_floats(*bad) == 0
+
+
+def test_hold_and_restore_refuse(hip_lib):
+    L = hip_lib
+    assert L.d3d_act8_hold(1, 64, 10, 64, 7, 0, 16, 1, None) == -1 and b"dtype" in err(L)
+    assert L.d3d_act8_hold(1, 64, 10, 64, 0, 2, 16, 1, None) == -1 and b"format" in err(L)
+    assert L.d3d_act8_hold(1, 64, -1, 64, 0, 0, 16, 1, None) == -1 and b"rows" in err(L)
+    assert L.d3d_act8_hold(1, 64, 10, 0, 0, 0, 16, 1, None) == -1
+    assert L.d3d_act8_hold(1, 63, 10, 64, 0, 0, 16, 1, None) == -1 and b"apart" in err(L)
+    assert L.d3d_act8_hold(None, 64, 10, 64, 0, 0, 16, 1, None) == -1 and b"null" in err(L)
+    assert L.d3d_act8_hold(1, 64, 10, 64, 0, 0, 8, 1, None) == -1 and b"aligned" in err(L)
+    assert L.d3d_act8_hold(None, 64, 0, 64, 0, 0, None, None, None) == 0  # no rows: nothing to do
+    assert L.d3d_act8_restore(16, 1, 10, 64, 0, 5, 1, 64, None) == -1 and b"dtype" in err(L)
+    assert L.d3d_act8_restore(16, None, 10, 64, 0, 0, 1, 64, None) == -1 and b"null" in err(L)
+    assert L.d3d_act8_restore(16, 1, 10, 64, 0, 0, 1, 60, None) == -1 and b"apart" in err(L)
+
+
+def test_weight_gradient_refuses(hip_lib):
+    L = hip_lib
+
+    def call(fmt=0, n_in=10, cin=64, stride=64, dtype=0, n_out=10, cout=64, nbr=1, cap=10, kvol=27, ws=16, wsb=1 << 40, dy=1):
+        return L.d3d_act8_wgrad(16, 1, fmt, n_in, cin, dy, stride, dtype, n_out, cout, nbr, cap, kvol, 1, ws, wsb, None)
+
+    assert call(fmt=3) == -1 and b"format" in err(L)
+    assert call(dtype=4) == -1 and b"dtype" in err(L)
+    assert call(n_in=0) == -1 and b"n_in" in err(L)
+    assert call(n_out=0) == -1
+    assert call(cap=9) == -1 and b"cap" in err(L)
+    assert call(nbr=None) == -1 and b"kvol" in err(L)
+    assert call(nbr=None, kvol=1, n_out=9) == -1
+    assert call(kvol=5000) == -1 and b"kvol" in err(L)
+    assert call(cin=20000, cout=20000, stride=20000) == -1 and b"weight of" in err(L)
+    assert call(stride=63) == -1 and b"apart" in err(L)
+    assert call(dy=None) == -1 and b"null" in err(L)
+    need = L.d3d_act8_wgrad_workspace_bytes(100000, 27, 64, 64, 0)
+    assert need > 0 and call(n_in=100000, n_out=100000, cap=100000, wsb=need - 1) == -2 and b"workspace" in err(L)
+
+
+def test_row_join_refuses(hip_lib):
+    from det3d_amd import _lib
+
+    L = hip_lib
+
+    def fwd(**kw):
+        a = dict(n=10, c=64, dtype=0, fmt=0, x=16, x_stride=64, f=16, f_stride=64, pre_kind=1, post_kind=1, h=16, z=16)
+        a.update(kw)
+        return L.d3d_row_join_fwd(ctypes.byref(_lib.RowJoin(**a)), None)
+
+    for kw, word in ((dict(dtype=2), b"dtype"), (dict(fmt=2), b"format"), (dict(n=0), b"rows"), (dict(c=8193), b"channels"), (dict(x=None), b"no rows"),
+                     (dict(x_stride=63), b"x rows"), (dict(f_stride=63), b"f rows"), (dict(x_codes=16), b"codes"), (dict(pre_kind=3), b"kinds"),
+                     (dict(pre_eps=-1.0), b"eps"), (dict(pre_eps=float("nan")), b"eps"), (dict(f=None), b"pre norm alone"), (dict(gate=16, gate_cols=5, gate_stride=5), b"gate"),
+                     (dict(gate=16, gate_cols=64, gate_stride=5), b"gate"), (dict(gate_act=3), b"gate_act"), (dict(h=None), b"null output"), (dict(z=None), b"null output"),
+                     (dict(x_codes=16, x_scales=1), b"together"), (dict(x_codes=8, x_scales=1, f_codes=16, f_scales=1), b"aligned")):
+        assert fwd(**kw) == -1 and word in err(L), (kw, err(L))
+    assert L.d3d_row_join_fwd(None, None) == -1
+
+    def bwd(a, **kw):
+        args = dict(n=10, c=64, dtype=0, fmt=0, x=16, x_stride=64, f=16, f_stride=64, pre_kind=1, post_kind=1)
+        args.update(a)
+        g = dict(dh=16, dh_stride=64, dz=16, dz_stride=64, dx=16, df=16)
+        g.update(kw)
+        return L.d3d_row_join_bwd(ctypes.byref(_lib.RowJoin(**args)), ctypes.byref(_lib.RowJoinGrads(**g)), None)
+
+    for a, kw, word in ((dict(), dict(dh_stride=63), b"dh rows"), (dict(), dict(dz_stride=63), b"dz rows"), (dict(pre_kind=0), dict(), b"without a pre"),
+                        (dict(f=None, post_kind=0), dict(df=None), b"without f"), (dict(), dict(dgate=16), b"without a gate"),
+                        (dict(), dict(dscale=16), b"absent vector"), (dict(x_codes=16, x_scales=1), dict(), b"f is not"),
+                        (dict(scale=16, n=100000), dict(dscale=16), None)):
+        rc = bwd(a, **kw)
+        assert (rc == -1 and word in err(L)) if word else (rc == -2 and b"workspace" in err(L)), (a, kw, err(L))
+
+
+def test_python_layer_without_a_gpu():
+    from det3d_amd import _lib, act8, rownorm
+
+    x = torch.zeros(4, 32)
+    with pytest.raises(_lib.D3dError, match="GPU only"):
+        act8.hold(x)
+    with pytest.raises(ValueError, match="format"):
+        act8.hold(x, "int7")
+    m = rownorm.RowNorm(32)
+    with pytest.raises(_lib.D3dError, match="GPU only"):
+        m(x)
+    with pytest.raises(_lib.D3dError, match="GPU only"):
+        rownorm.join(x, x, pre=m)
+    assert m.bias is None and rownorm.RowNorm(32, kind="layer").bias is not None and rownorm.RowNorm(8, affine=False).weight is None
+    assert [k for k, _ in rownorm.RowNorm(32, kind="layer").named_parameters()] == ["weight", "bias"]
+    for bad in (dict(num_features=0), dict(num_features=8193), dict(num_features=8, kind="group")):
+        with pytest.raises(ValueError):
+            rownorm.RowNorm(**bad)

@@ -12,9 +12,10 @@ import numpy as np
 import torch
 from torch import nn
 
-from . import spconv
+from . import rownorm, runtime, spconv
 from .nn_utils import build_norm_layer
 from .registry import BACKBONES
+from .rownorm import RowNorm
 from .spconv import SparseConv3d, SubMConv3d
 
 
@@ -77,6 +78,12 @@ class SparseBasicBlock(spconv.SparseModule):
             out.features = _bn_act(self.bn1, out.features, self.relu)
         if spconv.FUSE_BN_RELU and n != 0 and spconv._fusable_bn(self.bn2, out.features, channels=self.conv2.out_channels):
             out, _ = spconv.conv_bn_relu(self.conv2, self.bn2, False, out, link_in=link)
+        elif type(self.bn2) is RowNorm:
+            # a row norm: joined with the identity branch in one pass
+            out = self.conv2(out)
+            identity = x if self.downsample is None else self.downsample(x)
+            out.features = self.relu(rownorm.join(identity.features, out.features, post=self.bn2, checkpoint=runtime.held_format()))
+            return out
         else:
             out = self.conv2(out)
             out.features = self.bn2(out.features)

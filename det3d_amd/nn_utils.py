@@ -1,9 +1,11 @@
 """Small nn helpers with the reference's names and call signatures (API surface only; the bodies are this repo's):
-  build_norm_layer(cfg, n) -> (name, layer)   det3d/models/utils/norm.py:60-112   (config key "type": BN | BN1d | GN | SyncBN)
+  build_norm_layer(cfg, n) -> (name, layer)   det3d/models/utils/norm.py:60-112   (config key "type": BN | BN1d | GN | SyncBN,
+                                                                                   and this framework's row norms RMS | LN)
   Sequential(.add) with "0", "1", ... child names, Empty                          det3d/models/utils/misc.py:40-113
   get_paddings_indicator(actual_num, max_num)                                      det3d/models/utils/misc.py:180-202
 `Sequential.forward` is where the RPN's conv -> BN -> ReLU runs are handed to the library's kernels (dense_stack.py).
 """
+import functools
 import os
 from collections import OrderedDict
 
@@ -11,6 +13,7 @@ import torch
 from torch import nn
 
 
+from .rownorm import RowNorm
 from .syncbn import DistributedSyncBN  # noqa: E402  (reference semantics, det3d/ops/syncbn/syncbn.py)
 
 
@@ -20,6 +23,9 @@ norm_cfg = {
     "BN1d": ("bn1d", nn.BatchNorm1d),
     "GN": ("gn", nn.GroupNorm),
     "SyncBN": ("bn", DistributedSyncBN),
+    # norms of a row over its channels (rownorm.py): no batch statistics, hence no `momentum` and nothing to exchange over ranks
+    "RMS": ("rms", functools.partial(RowNorm, kind="rms")),
+    "LN": ("ln", functools.partial(RowNorm, kind="layer")),
 }
 
 

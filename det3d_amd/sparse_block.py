@@ -29,7 +29,7 @@ import os
 import torch
 from torch import nn
 
-from . import _lib, arena as mem, repack, syncbn
+from . import _lib, arena as mem, repack, runtime, syncbn
 
 FUSE_BLOCK = os.environ.get("D3D_FUSE_BLOCK", "1") != "0"
 
@@ -48,7 +48,7 @@ def _plain_bn(bn, c):
 
 def rulebook_of(sp, block, x):
     """the submanifold rulebook both convs of `block` share, if the block can run fused on `x`; else None"""
-    if not (FUSE_BLOCK and sp.FUSE_BN_RELU and sp.FUSE_BN_STATS) or block.downsample is not None:
+    if not (FUSE_BLOCK and sp.FUSE_BN_RELU and sp.FUSE_BN_STATS) or block.downsample is not None or runtime.held_format():
         return None
     c1, c2 = block.conv1, block.conv2
     feats = x.features

@@ -25,7 +25,7 @@ import numpy as np
 import torch
 from torch import nn
 
-from . import _lib, arena as mem, sparse_stack
+from . import _lib, act8, arena as mem, sparse_stack
 
 _SELF = sys.modules[__name__]
 _DT = {torch.float32: _lib.D3D_F32, torch.bfloat16: _lib.D3D_BF16}
@@ -486,7 +486,14 @@ class _SparseConvFn(torch.autograd.Function):
         rc = launch_fwd(rb, feats, wpack, b, pad_cin, cout, out, ep, _lib.stream_ptr(feats.device))
         _lib.check(rc, "d3d_sparse_conv_fwd")
         ctx.stats_done = ep is not None
-        ctx.save_for_backward(feats, weight)
+        fmt = _runtime.held_format()
+        ctx.feat_dtype, ctx.held = feats.dtype, None
+        if fmt is not None and ctx.needs_input_grad[1]:  # the weight gradient alone reads the input rows: keep them in 8 bits
+            held = act8.hold(feats, fmt)
+            ctx.save_for_backward(held.codes, held.scales, weight)
+            ctx.held = held.meta()
+        else:
+            ctx.save_for_backward(feats, None, weight)
         ctx.wd = wd
         from . import repack
         ctx.repack_stamp = repack.stamp((weight,))  # `wd` is rewritten in place by Repacker.run()
@@ -502,14 +509,15 @@ class _SparseConvFn(torch.autograd.Function):
     @_lib.ctx_backward
     def backward(ctx, gout):
         L = _lib.lib()
-        feats, weight = ctx.saved_tensors
+        feats, scales, weight = ctx.saved_tensors  # (held in 8 bits: codes, scales, weight)
         rb = ctx.rb
         kvol, cout = rb.kvol, weight.shape[-1]
         cin, pad_cin = ctx.pad
-        gout = gout.contiguous().to(feats.dtype)
+        feat_dtype, dev = ctx.feat_dtype, gout.device
+        gout = gout.contiguous().to(feat_dtype)
         check_gather_source(gout, "the output gradient")
-        dt = _DT[feats.dtype]
-        stream = _lib.stream_ptr(feats.device)
+        dt = _DT[feat_dtype]
+        stream = _lib.stream_ptr(dev)
         A = ctx.lease.check("sparse conv")
         gin = gw = gb = None
         if ctx.needs_input_grad[0]:
@@ -517,10 +525,10 @@ class _SparseConvFn(torch.autograd.Function):
             repack.check(ctx.repack_stamp, "sparse conv")
             wd = ctx.wd  # packed in the forward: W[k] as is; k mirrored for submanifold layers because
             #              (j -> i at offset k)  <=>  (i -> j at offset kvol-1-k) on the same table
-            gin = mem.empty((rb.n_in, pad_cin), feats.dtype, feats.device, A)
+            gin = mem.empty((rb.n_in, pad_cin), feat_dtype, dev, A)
             ep = None
             link = ctx.link
-            if link is not None and has_epilogue(cout, pad_cin, feats.dtype) and pad_cin == cin and rb.n_in > 0 and \
+            if link is not None and has_epilogue(cout, pad_cin, feat_dtype) and pad_cin == cin and rb.n_in > 0 and \
                     link.generation == ARENA.generation and not link.reduced and link.partial is not None:
                 # gin is dL/dy of the BN(+ReLU) that produced `feats`: reduce its gradient sums here
                 ep = _lib.ConvEpilogue(bn_x=link.x.data_ptr(), bn_mean=link.save[0].data_ptr(),
@@ -533,13 +541,18 @@ class _SparseConvFn(torch.autograd.Function):
             if pad_cin != cin:
                 gin = gin[:, :cin].contiguous()
         if ctx.needs_input_grad[1]:
-            gw = torch.empty((kvol, pad_cin, cout), dtype=torch.float32, device=feats.device)
-            wsb = L.d3d_sparse_conv_wgrad_workspace_bytes(rb.n_out, kvol, pad_cin, cout, dt)
-            ws = mem.empty((wsb,), torch.uint8, feats.device, A)
-            rc = _timed("wgrad", pad_cin, cout, rb.n_out, rb, feats.device, lambda: L.d3d_sparse_conv_wgrad(
-                feats.data_ptr(), gout.data_ptr(), rb.nbr_out.data_ptr(), rb.cap_out, rb.n_out, kvol,
-                pad_cin, cout, dt, gw.data_ptr(), ws.data_ptr(), wsb, stream))
-            _lib.check(rc, "d3d_sparse_conv_wgrad")
+            gw = torch.empty((kvol, pad_cin, cout), dtype=torch.float32, device=dev)
+            if ctx.held is not None:
+                held = act8.Held(feats, scales, *ctx.held)
+                _timed("wgrad", pad_cin, cout, rb.n_out, rb, dev, lambda: act8.launch_weight_grad(
+                    held, gout, rb.nbr_out.data_ptr(), rb.cap_out, kvol, gw))
+            else:
+                wsb = L.d3d_sparse_conv_wgrad_workspace_bytes(rb.n_out, kvol, pad_cin, cout, dt)
+                ws = mem.empty((wsb,), torch.uint8, dev, A)
+                rc = _timed("wgrad", pad_cin, cout, rb.n_out, rb, dev, lambda: L.d3d_sparse_conv_wgrad(
+                    feats.data_ptr(), gout.data_ptr(), rb.nbr_out.data_ptr(), rb.cap_out, rb.n_out, kvol,
+                    pad_cin, cout, dt, gw.data_ptr(), ws.data_ptr(), wsb, stream))
+                _lib.check(rc, "d3d_sparse_conv_wgrad")
             if pad_cin != cin:
                 gw = gw[:, :cin]
             gw = gw.reshape(weight.shape).to(weight.dtype)
@@ -573,7 +586,14 @@ class _BNReLUFn(torch.autograd.Function):
                             int(training), int(relu), _lib.ptr(stats) if training else None, copies, y.data_ptr(),
                             save[0].data_ptr(), save[1].data_ptr(), st)
         _lib.check(rc, "d3d_bn_apply")
-        ctx.save_for_backward(x, weight, bias, save)
+        # in 8 bits the backward sweeps read the restored rows (with the statistics of the full ones)
+        fmt, ctx.held = _runtime.held_format(), None
+        if fmt is not None and training and link is None and any(ctx.needs_input_grad[:3]):
+            held = act8.hold(x, fmt)
+            ctx.save_for_backward(held.codes, held.scales, weight, bias, save)
+            ctx.held = held.meta()
+        else:
+            ctx.save_for_backward(x, None, weight, bias, save)
         ctx.relu = relu
         ctx.training = training
         ctx.link = link
@@ -591,7 +611,9 @@ class _BNReLUFn(torch.autograd.Function):
         if not ctx.training:
             raise _lib.D3dError("fused sparse BN backward is implemented for training mode only")
         L = _lib.lib()
-        x, weight, bias, save = ctx.saved_tensors
+        x, scales, weight, bias, save = ctx.saved_tensors
+        if ctx.held is not None:
+            x = act8.Held(x, scales, *ctx.held).restore()
         n, c = x.shape
         dy = dy.contiguous().to(x.dtype)
         A = ctx.lease.check("sparse BatchNorm")
@@ -657,7 +679,8 @@ def conv_bn_relu(conv, bn, relu, x, link_in=None, want_link=False):
         stats = True  # the conv takes an epilogue_ws() slice once it knows its output row count
     out = conv(x, stats=stats, link=link_in if FUSE_BN_STATS else None)
     stats = getattr(out, "_stats", None)
-    link = _BnLink() if (want_link and fuse) else None
+    # (a link keeps the full pre-BN rows for the consuming conv's data gradient)
+    link = _BnLink() if (want_link and fuse and _runtime.held_format() is None) else None
     out.features = bn_relu(bn, out.features, relu, stats, link)
     return out, link
 
@@ -914,7 +937,8 @@ class SparseSequential(SparseModule):
         mods = list(self._modules.values())
         i = 0
         link = None  # _BnLink of the fused BN whose output is `input.features` (if this stack produced it)
-        stack_ok = FUSE_BN_RELU and FUSE_BN_STATS and sparse_stack.FUSE_STACK and torch.is_grad_enabled()
+        stack_ok = FUSE_BN_RELU and FUSE_BN_STATS and sparse_stack.FUSE_STACK and torch.is_grad_enabled() and \
+            _runtime.held_format() is None
         while i < len(mods):
             module = mods[i]
             if stack_ok and isinstance(module, SparseConvolution) and isinstance(input, SparseConvTensor) and \

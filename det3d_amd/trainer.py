@@ -122,11 +122,12 @@ class TrainStep:
         """one optimizer step on `example`.  after_forward: called between the forward and the backward enqueue -- the
         place to start host work for a LATER step (the next geometry build on its worker thread): the forward phase is
         the host-bound part of the step, the backward's large dense kernels leave the host time to spare."""
-        from . import arena
+        from . import arena, runtime
 
         A = None
         dev = self.params[0].device
-        if self.step_arena and dev.type == "cuda":
+        # (rows held in 8 bits: the full ones are to be freed as the forward pass goes on; an arena keeps all of them)
+        if self.step_arena and dev.type == "cuda" and runtime.held_format() is None:
             A = arena.step_arena(dev).begin()
         with arena.bound(A):
             return self._step(example, after_forward)

@@ -105,52 +105,315 @@ extern "C" int d3d_act8_restore(const uint8_t *codes, const uint8_t *scales, int
 }
 
 // ---- weight gradient: dW[k][ci][co] = sum_o x[nbr[k][o]][ci] dy[o][co]
-// A thread owns one (ci, co) of a 16 x 16 tile and walks the rows of its split; the splits' sums go to the workspace and are
-// added in split order.
-template <bool BF16, int FMT>
-__global__ void __launch_bounds__(256)
-    a8_wgrad_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t n_in, int cin, int pitch,
-                    const void *__restrict__ dy, int64_t dy_stride, int64_t n_out, int cout, const int32_t *__restrict__ nbr,
-                    int64_t cap, int64_t rows_per_split, float *__restrict__ part, int64_t part_stride) {
-  const int tiles_co = (cout + 15) / 16, tiles_ci = (cin + 15) / 16;
-  const int co = (blockIdx.x % tiles_co) * 16 + (threadIdx.x & 15);
-  const int ci = (blockIdx.x / tiles_co % tiles_ci) * 16 + (threadIdx.x >> 4);
-  const int k = blockIdx.x / (tiles_co * tiles_ci);
-  if (ci >= cin || co >= cout) return;
-  const int64_t first = blockIdx.y * rows_per_split;
-  const int64_t last = first + rows_per_split < n_out ? first + rows_per_split : n_out;
-  float sum = 0.f;
-  for (int64_t o = first; o < last; ++o) {
-    const int64_t i = nbr ? nbr[k * cap + o] : o;
-    if (i < 0 || i >= n_in) continue;
-    float x, g;
-    A8Held<FMT, 1, 32>::load(codes, scales, i, pitch, ci, &x);
-    A8Row<BF16, 1>::load(dy, o * dy_stride + co, &g);
-    sum = fmaf(x, g, sum);
+//
+// A matrix product whose long axis, the rows o, is the outer one of both operands; bound by the matrix pipe for float32 dy and by
+// LDS / the gathers for bf16.  The (k, ci) axis is flattened (ci padded to 8) and cut into units of 64 columns, so narrow layers
+// fill a unit with several offsets.  A block of 8 waves owns KG units x TN columns of dy and a range of rows, 64 rows (a chunk)
+// at a time:
+//   * dy's chunk goes through LDS once, as P bf16 planes (f32: three, hi + mid + lo = all 24 bits; restored values are exact in
+//     bf16, so the products are exact to f32 either way), and stays in registers as the MFMA's B operand for all KG units;
+//   * a unit's 64 x 64 codes are one 8-byte gather a thread, requested a whole chunk (KG units) ahead, its table entry a chunk
+//     further; restored to bf16 on the way into LDS (double buffered, one barrier a unit);
+//   * both operands become MFMA fragments, rows as k, through the transposing read ds_read_b64_tr_b16.
+// Wave (wci, wco, wk): 32 of the unit's columns, 32 NB of dy's, every WK-th part of the chunk's rows; the wk parts are added in
+// the block, the row ranges through the workspace in their order.
+typedef __attribute__((ext_vector_type(4))) short a8_s16x4;
+typedef __attribute__((ext_vector_type(8))) short a8_s16x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 a8_bf16x8;
+typedef __attribute__((ext_vector_type(16))) float a8_f32x16;
+
+#define WG8_ROWS 64
+
+struct Wg8Args {
+  const uint8_t *codes, *scales;
+  const void *dy;
+  const int32_t *nbr;
+  float *out;  // [splits][kvol][cin][cout], or dw itself
+  int64_t dy_stride, cap, count;
+  uint32_t n_in;
+  int n_out, cin, cinp, pitch, cout, cols, units, groups, cotiles, chunks, per_split, vec;
+};
+
+template <int FMT> __device__ __forceinline__ uint4 wg8_restore(uint2 w, uint32_t b) {
+  // 8 codes to bf16: exact, so the upper halves of the f32 values are taken as they are
+  const float s = a8_up(b);
+  uint32_t v[8];
+  if constexpr (FMT == D3D_ACT8_INT8) {
+    // biased to unsigned bytes, whose conversion is one instruction: (code + 128) 2^s - 128 2^s
+    const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
+    const float m = -128.f * s;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = __float_as_uint(fmaf((float)((x >> (8 * j)) & 0xffu), s, m));
+      v[4 + j] = __float_as_uint(fmaf((float)((y >> (8 * j)) & 0xffu), s, m));
+    }
+  } else {
+    float f[8];
+    a8_value4<FMT>(w.x, s, f);
+    a8_value4<FMT>(w.y, s, f + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(f[j]);
   }
-  part[blockIdx.y * part_stride + ((int64_t)k * cin + ci) * cout + co] = sum;
+  return make_uint4(__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u),
+                    __builtin_amdgcn_perm(v[5], v[4], 0x07060302u), __builtin_amdgcn_perm(v[7], v[6], 0x07060302u));
 }
 
-__global__ void __launch_bounds__(256)
-    a8_fold_kernel(const float *__restrict__ part, int64_t count, int splits, float *__restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (int p = 0; p < splits; ++p) s += part[p * count + i];
-    out[i] = s;
+// byte of 16-byte slot `slot` in row r of a [rows][W columns] bf16 tile.  The slots of a row are permuted so that the four rows
+// of a transposing read (64 bytes each) lie in different banks: 128-byte rows alternate halves every second row, wider ones
+// rotate quarters of 256 bytes
+template <int W> __device__ __forceinline__ uint32_t wg8_slot(int r, int slot) {
+  if constexpr (W == 64) slot ^= ((r >> 1) & 1) << 2;
+  if constexpr (W >= 128) slot ^= (r & 3) << 2;
+  return (uint32_t)(r * (W * 2) + slot * 16);
+}
+
+// fragment of mfma_f32_32x32x16_bf16: columns [col, col + 32), rows [row, row + 16) of such a tile; lane l holds column l % 32,
+// rows 8 (l / 32) + 0 .. 7
+template <int W> __device__ __forceinline__ a8_bf16x8 wg8_fragment(const unsigned char *tile, int row, int col) {
+  const int lane = threadIdx.x & 63, i16 = lane & 15;
+  const int r = row + ((lane >> 5) << 3) + (i16 >> 2);
+  const int c = col + (((lane >> 4) & 1) << 4) + ((i16 & 3) << 2);
+  typedef __attribute__((address_space(3))) a8_s16x4 lds_s16x4;
+  const unsigned char *p = tile + wg8_slot<W>(r, c >> 3) + (c & 7) * 2;  // (row r + 4 has the same permutation)
+  const a8_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+  const a8_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * W * 2));
+  const a8_s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(a8_bf16x8, v);
+}
+
+template <int FMT, int P, int WCO, int WK, int NB, int KG, bool TABLE>
+__global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
+  constexpr int TN = WCO * NB * 32, KS = WG8_ROWS / WK / 16;
+  constexpr int VPT = TN >= 64 ? TN / 64 : 1;  // vectors of 8 columns of dy a thread stages
+  constexpr int ABYTES = WG8_ROWS * 128, DBYTES = WG8_ROWS * TN * 2;
+  constexpr int RBYTES = (WK - 1) * 2 * WCO * 4096;
+  constexpr int SMEM = 2 * ABYTES + P * DBYTES > RBYTES ? 2 * ABYTES + P * DBYTES : RBYTES;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[SMEM];
+  unsigned char *const sa = smem, *const sd = smem + 2 * ABYTES;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wci = wave & 1, wco = (wave >> 1) % WCO, wk = (wave >> 1) / WCO;
+  // blocks of one row range next to each other on one XCD: they read the same rows of dy and the same codes
+  int logical;
+  {
+    const int nb = (int)gridDim.x, q = nb >> 3, r = nb & 7, xcd = (int)blockIdx.x & 7, idx = (int)blockIdx.x >> 3;
+    logical = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  }
+  const int cot = logical % p.cotiles, group = logical / p.cotiles % p.groups, split = logical / (p.cotiles * p.groups);
+  const int co0 = cot * TN, unit0 = group * KG;
+  const int nu = p.units - unit0 < KG ? p.units - unit0 : KG;
+  const int chunk0 = split * p.per_split;
+  const int chunks = p.chunks - chunk0 < p.per_split ? p.chunks - chunk0 : p.per_split;
+
+  // this thread's 8 columns of each unit, and its row of the chunk
+  const int srow = tid >> 3, sseg = tid & 7;
+  int ci[KG], tab[KG];  // column within the row of codes (-1: behind the last column) | offset k
+#pragma unroll
+  for (int u = 0; u < KG; ++u) {
+    const int col = (unit0 + u) * 64 + sseg * 8;
+    const bool in = u < nu && col < p.cols;
+    tab[u] = TABLE && in ? col / p.cinp : 0;
+    ci[u] = in ? col - tab[u] * p.cinp : -1;
+  }
+  int32_t idx[KG];
+  uint2 code[KG];
+  uint32_t sc[KG];
+  auto load_idx = [&](int u, int chunk) {  // rows behind the last and columns behind the last: absent
+    const int o = (chunk0 + chunk) * WG8_ROWS + srow;
+    idx[u] = -1;
+    if (chunk < chunks && o < p.n_out && ci[u] >= 0) idx[u] = TABLE ? p.nbr[tab[u] * p.cap + o] : o;
+  };
+  auto load_code = [&](int u) {
+    const bool in = (uint32_t)idx[u] < p.n_in;
+    const int64_t row = in ? idx[u] : 0;
+    const int c = in ? ci[u] : 0;
+    code[u] = *(const uint2 *)(p.codes + row * p.pitch + c);
+    const uint32_t b = p.scales[row * (p.pitch >> 5) + (c >> 5)];
+    sc[u] = in ? b : 0u;  // scale 0: the row adds nothing
+  };
+
+  // dy: thread's vectors of the chunk
+  float dyv[P == 3 ? VPT * 8 : 1];
+  uint4 dyb[P == 3 ? 1 : VPT];
+  auto load_dy = [&](int chunk) {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int i = tid + 512 * v, r = i / (TN / 8), cv = i % (TN / 8);
+      const int o = (chunk0 + chunk) * WG8_ROWS + r, co = co0 + cv * 8;
+      const bool in = r < WG8_ROWS && o < p.n_out && co < p.cout;
+      if constexpr (P == 3) {
+        const float *src = (const float *)p.dy + (int64_t)(in ? o : 0) * p.dy_stride;
+        if (p.vec && co + 8 <= p.cout) {
+          const float4 x = in ? *(const float4 *)(src + co) : make_float4(0, 0, 0, 0);
+          const float4 y = in ? *(const float4 *)(src + co + 4) : make_float4(0, 0, 0, 0);
+          dyv[v * 8] = x.x; dyv[v * 8 + 1] = x.y; dyv[v * 8 + 2] = x.z; dyv[v * 8 + 3] = x.w;
+          dyv[v * 8 + 4] = y.x; dyv[v * 8 + 5] = y.y; dyv[v * 8 + 6] = y.z; dyv[v * 8 + 7] = y.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dyv[v * 8 + j] = in && co + j < p.cout ? src[co + j] : 0.f;
+        }
+      } else {
+        const uint16_t *src = (const uint16_t *)p.dy + (int64_t)(in ? o : 0) * p.dy_stride;
+        if (p.vec && co + 8 <= p.cout) {
+          dyb[v] = in ? *(const uint4 *)(src + co) : make_uint4(0, 0, 0, 0);
+        } else {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = in && co + j < p.cout ? src[co + j] : 0u;
+          dyb[v] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        }
+      }
+    }
+  };
+  auto write_dy = [&]() {
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int i = tid + 512 * v, r = i / (TN / 8), cv = i % (TN / 8);
+      if (r >= WG8_ROWS) continue;
+      const uint32_t at = wg8_slot<TN>(r, cv);
+      if constexpr (P == 3) {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a = dyv[v * 8 + 2 * j], b = dyv[v * 8 + 2 * j + 1];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) {  // bf16 of what is left, and what that leaves (exact)
+            w[q][j] = a8_pack_bf16(a, b);
+            a -= __uint_as_float(w[q][j] << 16);
+            b -= __uint_as_float(w[q][j] & 0xffff0000u);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *(uint4 *)(sd + q * DBYTES + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+      } else {
+        *(uint4 *)(sd + at) = dyb[v];
+      }
+    }
+  };
+
+  a8_f32x16 acc[KG][NB];
+#pragma unroll
+  for (int u = 0; u < KG; ++u)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[u][n][r] = 0.f;
+
+#pragma unroll
+  for (int u = 0; u < KG; ++u) load_idx(u, 0);
+  load_dy(0);
+#pragma unroll
+  for (int u = 0; u < KG; ++u) {
+    load_code(u);
+    load_idx(u, 1);
+  }
+  for (int chunk = 0; chunk < chunks; ++chunk) {
+    auto stage = [&](int u) {
+      *(uint4 *)(sa + (u & 1) * ABYTES + wg8_slot<64>(srow, sseg)) = wg8_restore<FMT>(code[u], sc[u]);
+      load_code(u);  // of the next chunk (its index arrived a chunk ago)
+      load_idx(u, chunk + 2);
+    };
+    write_dy();
+    stage(0);
+    d3d_lds_barrier();
+    a8_bf16x8 bf[KS][NB][P];
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int q = 0; q < P; ++q) bf[k][n][q] = wg8_fragment<TN>(sd + q * DBYTES, (wk * KS + k) * 16, (wco * NB + n) * 32);
+    if (chunk + 1 < chunks) load_dy(chunk + 1);
+#pragma unroll
+    for (int u = 0; u < KG; ++u) {
+      if (u < nu) {
+        if (u + 1 < KG && u + 1 < nu) stage(u + 1);
+        a8_bf16x8 af[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) af[k] = wg8_fragment<64>(sa + (u & 1) * ABYTES, (wk * KS + k) * 16, wci * 32);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int q = P - 1; q >= 0; --q) acc[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[k], bf[k][n][q], acc[u][n], 0, 0, 0);
+        d3d_lds_barrier();
+      }
+    }
+  }
+
+  // ---- the parts of the chunk's rows (wk) together, then out: lane l holds column l % 32 of dy's 32, rows 8 (r / 4) + 4 (l / 32) + r % 4
+#pragma unroll
+  for (int u = 0; u < KG; ++u) {
+    if (u >= nu) continue;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      if constexpr (WK > 1) {
+        float *red = (float *)smem;
+        if (wk > 0) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) red[(((wk - 1) * 2 * WCO + (wave & (2 * WCO - 1))) * 16 + r) * 64 + lane] = acc[u][n][r];
+        }
+        d3d_lds_barrier();
+        if (wk == 0) {
+#pragma unroll
+          for (int q = 0; q < WK - 1; ++q)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[u][n][r] += red[((q * 2 * WCO + wave) * 16 + r) * 64 + lane];
+        }
+        d3d_lds_barrier();
+        if (wk > 0) continue;
+      }
+      const int co = co0 + (wco * NB + n) * 32 + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int col = (unit0 + u) * 64 + wci * 32 + (r >> 2) * 8 + ((lane >> 5) << 2) + (r & 3);
+        const int k = col / p.cinp, c = col - k * p.cinp;
+        if (col < p.cols && c < p.cin && co < p.cout) p.out[split * p.count + ((int64_t)k * p.cin + c) * p.cout + co] = acc[u][n][r];
+      }
+    }
   }
 }
 
-static int a8_wgrad_splits(int64_t n_out, int kvol, int cin, int cout) {
-  const int64_t tiles = (int64_t)kvol * ((cin + 15) / 16) * ((cout + 15) / 16);
-  int64_t s = 4096 / tiles;
-  const int64_t most = (n_out + 63) / 64;
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : s);
+// the row ranges' sums in their order: four parts of the ranges side by side, then the parts
+__global__ void __launch_bounds__(256) a8_fold_kernel(const float *__restrict__ part, int64_t count, int splits, float *__restrict__ out) {
+  __shared__ float sum[4][64];
+  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int q = threadIdx.x >> 6, per = (splits + 3) / 4;
+  float s = 0.f;
+  if (i < count) {
+    const int last = (q + 1) * per < splits ? (q + 1) * per : splits;
+    for (int k = q * per; k < last; ++k) s += part[k * count + i];
+  }
+  sum[q][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (q == 0 && i < count) out[i] = (s + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
+}
+
+// how a weight gradient is cut: columns of dy a block, units, row ranges
+struct Wg8Plan {
+  int tn, units, groups, cotiles, chunks, per_split, splits;
+};
+#define WG8_KG 4
+static Wg8Plan wg8_plan(int64_t n_out, int kvol, int cin, int cout, int dtype) {
+  Wg8Plan q;
+  q.tn = cout <= 32 ? 32 : (cout <= 64 ? 64 : (cout <= 128 || dtype == D3D_F32 ? 128 : 256));
+  q.units = (int)(((int64_t)kvol * ((cin + 7) / 8 * 8) + 63) / 64);
+  q.groups = (q.units + WG8_KG - 1) / WG8_KG;
+  q.cotiles = (cout + q.tn - 1) / q.tn;
+  q.chunks = (int)((n_out + WG8_ROWS - 1) / WG8_ROWS);
+  const int64_t tiles = (int64_t)q.groups * q.cotiles;
+  int64_t s = 256 / tiles;
+  s = s < 1 ? 1 : (s > q.chunks ? q.chunks : s);
+  q.per_split = (int)((q.chunks + s - 1) / s);
+  q.splits = (q.chunks + q.per_split - 1) / q.per_split;
+  return q;
 }
 
 extern "C" size_t d3d_act8_wgrad_workspace_bytes(int64_t n_out, int kvol, int cin, int cout, int dtype) {
   if (n_out < 1 || kvol < 1 || cin < 1 || cout < 1 || (dtype != D3D_F32 && dtype != D3D_BF16)) return 0;
-  const int splits = a8_wgrad_splits(n_out, kvol, cin, cout);
+  const int splits = wg8_plan(n_out, kvol, cin, cout, dtype).splits;
   return splits > 1 ? (size_t)splits * kvol * cin * cout * sizeof(float) : 0;
 }
 
@@ -163,8 +426,8 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   D3D_REQUIRE(n_in >= 1 && n_out >= 1, "d3d_act8_wgrad: n_in=%lld n_out=%lld (empty gradients are the caller's business)",
               (long long)n_in, (long long)n_out);
   D3D_REQUIRE(cout >= 1 && cout <= (1 << 20) && kvol >= 1 && kvol <= 4096, "d3d_act8_wgrad: cout=%d kvol=%d", cout, kvol);
-  D3D_REQUIRE((int64_t)kvol * cin * cout < ((int64_t)1 << 31), "d3d_act8_wgrad: a weight of %d x %d x %d", kvol, cin, cout);
-  D3D_REQUIRE(n_in < ((int64_t)1 << 31) && n_out < ((int64_t)1 << 31), "d3d_act8_wgrad: %lld / %lld rows", (long long)n_in, (long long)n_out);
+  D3D_REQUIRE((int64_t)kvol * cin * cout < ((int64_t)1 << 30), "d3d_act8_wgrad: a weight of %d x %d x %d", kvol, cin, cout);
+  D3D_REQUIRE(n_in < ((int64_t)1 << 31) - 4096 && n_out < ((int64_t)1 << 31) - 4096, "d3d_act8_wgrad: %lld / %lld rows", (long long)n_in, (long long)n_out);
   D3D_REQUIRE(codes && scales && dy && dw, "d3d_act8_wgrad: null pointer");
   D3D_REQUIRE(dy_stride >= cout, "d3d_act8_wgrad: rows of %d channels %lld elements apart", cout, (long long)dy_stride);
   D3D_REQUIRE(nbr ? cap >= n_out : (kvol == 1 && n_in == n_out), "d3d_act8_wgrad: cap=%lld kvol=%d n_in=%lld n_out=%lld",
@@ -172,18 +435,56 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   const size_t need = d3d_act8_wgrad_workspace_bytes(n_out, kvol, cin, cout, dtype);
   if (need && (!workspace || workspace_bytes < need))
     return d3d_set_error(D3D_ECAPACITY, "d3d_act8_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  const int splits = a8_wgrad_splits(n_out, kvol, cin, cout), pitch = a8_pitch(cin);
-  const int64_t count = (int64_t)kvol * cin * cout, per = (n_out + splits - 1) / splits;
-  float *part = splits > 1 ? (float *)workspace : dw;
-  const dim3 grid((unsigned)(kvol * ((cin + 15) / 16) * ((cout + 15) / 16)), (unsigned)splits);
-#define A8_WG(BF, F) hipLaunchKernelGGL((a8_wgrad_kernel<BF, F>), grid, dim3(256), 0, stream, codes, scales, n_in, cin, pitch, dy, \
-                                        dy_stride, n_out, cout, nbr, cap, per, part, count)
-  if (dtype == D3D_BF16) { if (fmt == D3D_ACT8_INT8) A8_WG(true, D3D_ACT8_INT8); else A8_WG(true, D3D_ACT8_E4M3); }
-  else { if (fmt == D3D_ACT8_INT8) A8_WG(false, D3D_ACT8_INT8); else A8_WG(false, D3D_ACT8_E4M3); }
+  const Wg8Plan q = wg8_plan(n_out, kvol, cin, cout, dtype);
+  Wg8Args p;
+  p.codes = codes;
+  p.scales = scales;
+  p.dy = dy;
+  p.nbr = nbr;
+  p.out = q.splits > 1 ? (float *)workspace : dw;
+  p.dy_stride = dy_stride;
+  p.cap = cap;
+  p.count = (int64_t)kvol * cin * cout;
+  p.n_in = (uint32_t)n_in;
+  p.n_out = (int)n_out;
+  p.cin = cin;
+  p.cinp = (cin + 7) / 8 * 8;
+  p.pitch = a8_pitch(cin);
+  p.cout = cout;
+  p.cols = kvol * p.cinp;
+  p.units = q.units;
+  p.groups = q.groups;
+  p.cotiles = q.cotiles;
+  p.chunks = q.chunks;
+  p.per_split = q.per_split;
+  p.vec = ((uintptr_t)dy & 15) == 0 && dy_stride % (dtype == D3D_BF16 ? 8 : 4) == 0;
+  const dim3 grid((unsigned)(q.groups * q.cotiles * q.splits));
+#define A8_WG(F, P, WCO, WK, NB)                                                                                                \
+  do {                                                                                                                          \
+    if (nbr) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, WG8_KG, true>), grid, dim3(512), 0, stream, p);             \
+    else hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, WG8_KG, false>), grid, dim3(512), 0, stream, p);                \
+  } while (0)
+#define A8_WG_TN(F)                                                                                                             \
+  do {                                                                                                                          \
+    if (dtype == D3D_BF16) {                                                                                                    \
+      if (q.tn == 32) A8_WG(F, 1, 1, 4, 1);                                                                                     \
+      else if (q.tn == 64) A8_WG(F, 1, 2, 2, 1);                                                                                \
+      else if (q.tn == 128) A8_WG(F, 1, 4, 1, 1);                                                                               \
+      else A8_WG(F, 1, 4, 1, 2);                                                                                                \
+    } else {                                                                                                                    \
+      if (q.tn == 32) A8_WG(F, 3, 1, 4, 1);                                                                                     \
+      else if (q.tn == 64) A8_WG(F, 3, 2, 2, 1);                                                                                \
+      else A8_WG(F, 3, 4, 1, 1);                                                                                                \
+    }                                                                                                                           \
+  } while (0)
+  if (fmt == D3D_ACT8_INT8) A8_WG_TN(D3D_ACT8_INT8);
+  else A8_WG_TN(D3D_ACT8_E4M3);
+#undef A8_WG_TN
 #undef A8_WG
   D3D_LAUNCH_TRY("a8_wgrad_kernel");
-  if (splits > 1) {
-    hipLaunchKernelGGL(a8_fold_kernel, dim3(a8_grid(count)), dim3(256), 0, stream, part, count, splits, dw);
+  if (q.splits > 1) {
+    hipLaunchKernelGGL(a8_fold_kernel, dim3((unsigned)((p.count + 63) / 64)), dim3(256), 0, stream, (const float *)workspace, p.count,
+                       q.splits, dw);
     D3D_LAUNCH_TRY("a8_fold_kernel");
   }
   return D3D_OK;

@@ -66,37 +66,50 @@ __device__ __forceinline__ uint32_t a8_pack_bf16(float a, float b) {  // round t
 }
 
 // E neighbouring values of a row in the feature type: one 16-byte access (E = 4 f32 / 8 bf16), or one value (E = 1) where the
-// row is not aligned to 16 bytes or its width is no multiple of E
+// row is not aligned to 16 bytes or its width is no multiple of E.  Raw is what a load leaves in registers: loads issued early
+// and unpacked late stay in flight in between.
 template <bool BF16, int E> struct A8Row {
   static_assert(E == 1 || E == (BF16 ? 8 : 4), "one value or one 16-byte vector");
-  __device__ static __forceinline__ void load(const void *row, int64_t at, float *v) {
+  struct Raw {
+    uint32_t w[E == 1 ? 1 : 4];
+  };
+  __device__ static __forceinline__ Raw fetch(const void *row, int64_t at) {
+    Raw r;
     if constexpr (E == 1) {
-      if constexpr (BF16) v[0] = __uint_as_float((uint32_t)((const uint16_t *)row)[at] << 16);
-      else v[0] = ((const float *)row)[at];
-    } else if constexpr (BF16) {
-      const uint4 r = *(const uint4 *)((const uint16_t *)row + at);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      if constexpr (BF16) r.w[0] = (uint32_t)((const uint16_t *)row)[at] << 16;
+      else r.w[0] = ((const uint32_t *)row)[at];
+    } else {
+      const uint4 q = *(const uint4 *)((const char *)row + at * (BF16 ? 2 : 4));
+      r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+    }
+    return r;
+  }
+  __device__ static __forceinline__ Raw zero() {
+    Raw r;
+#pragma unroll
+    for (uint32_t &w : r.w) w = 0u;
+    return r;
+  }
+  __device__ static __forceinline__ void unpack(const Raw &r, float *v) {
+    if constexpr (E > 1 && BF16) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        v[2 * j] = __uint_as_float(r.w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(r.w[j] & 0xffff0000u);
       }
     } else {
-      const float4 r = *(const float4 *)((const float *)row + at);
-      v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = __uint_as_float(r.w[j]);
     }
   }
+  __device__ static __forceinline__ void load(const void *row, int64_t at, float *v) { unpack(fetch(row, at), v); }
   __device__ static __forceinline__ void store(void *row, int64_t at, const float *v) {
     if constexpr (E == 1) {
       if constexpr (BF16) ((uint16_t *)row)[at] = (uint16_t)(a8_pack_bf16(v[0], 0.f) & 0xffffu);
       else ((float *)row)[at] = v[0];
     } else if constexpr (BF16) {
-      uint4 r;
-      r.x = a8_pack_bf16(v[0], v[1]);
-      r.y = a8_pack_bf16(v[2], v[3]);
-      r.z = a8_pack_bf16(v[4], v[5]);
-      r.w = a8_pack_bf16(v[6], v[7]);
-      *(uint4 *)((uint16_t *)row + at) = r;
+      *(uint4 *)((uint16_t *)row + at) =
+          make_uint4(a8_pack_bf16(v[0], v[1]), a8_pack_bf16(v[2], v[3]), a8_pack_bf16(v[4], v[5]), a8_pack_bf16(v[6], v[7]));
     } else {
       *(float4 *)((float *)row + at) = make_float4(v[0], v[1], v[2], v[3]);
     }
@@ -134,21 +147,43 @@ template <int FMT, int E, int LANES> struct A8Held {
     }
     if ((at & (A8_GROUP - 1)) == 0) scales[row * (pitch / A8_GROUP) + at / A8_GROUP] = (uint8_t)b;
   }
-  __device__ static __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t row, int pitch, int at,
-                                              float *v) {
-    const float up = a8_up(scales[row * (pitch / A8_GROUP) + at / A8_GROUP]);
+  struct Raw {
+    uint32_t w[E == 8 ? 2 : 1], b;
+  };
+  __device__ static __forceinline__ Raw fetch(const uint8_t *codes, const uint8_t *scales, int64_t row, int pitch, int at) {
+    Raw r;
+    r.b = scales[row * (pitch / A8_GROUP) + at / A8_GROUP];
     const uint8_t *c = codes + row * pitch + at;
+    if constexpr (E == 1) r.w[0] = *c;
+    else if constexpr (E == 4) r.w[0] = *(const uint32_t *)c;
+    else {
+      const uint2 q = *(const uint2 *)c;
+      r.w[0] = q.x;
+      r.w[1] = q.y;
+    }
+    return r;
+  }
+  __device__ static __forceinline__ Raw zero() {
+    Raw r;
+#pragma unroll
+    for (uint32_t &w : r.w) w = 0u;
+    r.b = 0u;
+    return r;
+  }
+  __device__ static __forceinline__ void unpack(const Raw &r, float *v) {
+    const float up = a8_up(r.b);
     if constexpr (E == 1) {
       float q[4];
-      a8_value4<FMT>(*c, up, q);
+      a8_value4<FMT>(r.w[0], up, q);
       v[0] = q[0];
-    } else if constexpr (E == 4) {
-      a8_value4<FMT>(*(const uint32_t *)c, up, v);
     } else {
-      const uint2 w = *(const uint2 *)c;
-      a8_value4<FMT>(w.x, up, v);
-      a8_value4<FMT>(w.y, up, v + 4);
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j) a8_value4<FMT>(r.w[j], up, v + 4 * j);
     }
+  }
+  __device__ static __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t row, int pitch, int at,
+                                              float *v) {
+    unpack(fetch(codes, scales, row, pitch, at), v);
   }
 };
 

@@ -12,6 +12,7 @@
 // codes) instead of reading saved ones.
 #include "d3d_act8.h"
 #include <string.h>
+#include <type_traits>
 
 
 template <int T, int NT, int N> __device__ __forceinline__ void row_sum(float *v, float (&lds)[2][N][NT / 64], int &slot) {
@@ -43,20 +44,9 @@ struct RjArgs {
   D3dRowJoinGrads g;
   float inv_c;
   int pitch;
-  float *part;     // backward: [blocks][sums][c] when the grid has more than one block, else null
+  float *part;  // backward: [blocks][sums][c] when the grid has more than one block, else null
   int sums;
 };
-
-__device__ __forceinline__ void rj_act(int act, float g, float &a, float &da) {
-  if (act == D3D_GATE_NONE) {
-    a = g;
-    da = 1.f;
-    return;
-  }
-  const float p = 1.f / (1.f + expf(-g));
-  a = act == D3D_GATE_SIGMOID ? p : g * p;
-  da = act == D3D_GATE_SIGMOID ? p * (1.f - p) : p * (1.f + g * (1.f - p));
-}
 
 // T lanes own a row, NV vectors of E values each; RPB rows to a block of NT threads
 template <bool BF16_, int E_, int T_, int NV_> struct RjShape {
@@ -65,50 +55,102 @@ template <bool BF16_, int E_, int T_, int NV_> struct RjShape {
   static constexpr int NT = T > 256 ? T : 256, RPB = NT / T, EPL = E * NV;
 };
 
-// (v - mu) and r of a row in place
-template <int T, int NT, int E, int NV>
-__device__ __forceinline__ float rj_normalise(int kind, float eps, float inv_c, int lane, int units, float *v,
-                                              float (&lds1)[2][1][NT / 64], int &slot) {
+// act(g) and, with DA, its derivative.  exp and reciprocal are the hardware's (one step off at most): 1 / (1 + 2^(-g log2 e))
+template <bool DA> __device__ __forceinline__ void rj_act(int act, float g, float &a, float &da) {
+  const float p = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
+  if (act == D3D_GATE_SIGMOID) {
+    a = p;
+    if constexpr (DA) da = fmaf(-p, p, p);
+  } else {
+    a = g * p;
+    if constexpr (DA) da = fmaf(a, 1.f - p, p);
+  }
+}
+
+// a [c] vector's values of this lane (`absent` where there is none), times `factor`; kept in registers over the rows
+template <class S> __device__ __forceinline__ void rj_vector(const float *w, float absent, float factor, int lane, int c, float *v) {
+#pragma unroll
+  for (int k = 0; k < S::NV; ++k) {
+    const int at = (k * S::T + lane) * S::E;
+#pragma unroll
+    for (int j = 0; j < S::E; ++j) v[k * S::E + j] = absent * factor;
+    if (w != nullptr && at < c) {
+      if constexpr (S::E == 1) v[k] = w[at] * factor;
+      else {
+#pragma unroll
+        for (int j = 0; j < S::E; j += 4) {
+          const float4 q = *(const float4 *)(w + at + j);
+          v[k * S::E + j] = q.x * factor;
+          v[k * S::E + j + 1] = q.y * factor;
+          v[k * S::E + j + 2] = q.z * factor;
+          v[k * S::E + j + 3] = q.w * factor;
+        }
+      }
+    }
+  }
+}
+
+// v - mu in place (layer) and r; values behind the row's end stay zero
+template <class S>
+__device__ __forceinline__ float rj_normalise(int kind, float eps, float inv_c, int lane, int c, float *v,
+                                              float (&lds1)[2][1][S::NT / 64], int &slot) {
   if (kind == D3D_NORM_LAYER) {
     float s[1] = {0.f};
 #pragma unroll
-    for (int j = 0; j < E * NV; ++j) s[0] += v[j];
-    row_sum<T, NT, 1>(s, lds1, slot);
+    for (int j = 0; j < S::EPL; ++j) s[0] += v[j];
+    row_sum<S::T, S::NT, 1>(s, lds1, slot);
     const float mu = s[0] * inv_c;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const bool in = k * T + lane < units;
+    for (int k = 0; k < S::NV; ++k) {
+      const float m = (k * S::T + lane) * S::E < c ? mu : 0.f;
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[k * E + j] = in ? v[k * E + j] - mu : 0.f;
+      for (int j = 0; j < S::E; ++j) v[k * S::E + j] -= m;
     }
   }
   float q[1] = {0.f};
 #pragma unroll
-  for (int j = 0; j < E * NV; ++j) q[0] = fmaf(v[j], v[j], q[0]);
-  row_sum<T, NT, 1>(q, lds1, slot);
-  return 1.f / sqrtf(fmaf(q[0], inv_c, eps));
+  for (int j = 0; j < S::EPL; ++j) q[0] = fmaf(v[j], v[j], q[0]);
+  row_sum<S::T, S::NT, 1>(q, lds1, slot);
+  return rsqrtf(fmaf(q[0], inv_c, eps));
 }
 
 template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fwd_kernel(RjArgs p) {
-  constexpr bool BF16 = S::BF16;
   constexpr int E = S::E, T = S::T, NV = S::NV;
   constexpr int GL = A8_GROUP / E < T ? A8_GROUP / E : T;
+  using Row = A8Row<S::BF16, E>;
   __shared__ float lds1[2][1][S::NT / 64];
   int slot = 0;
   const D3dRowJoin &a = p.a;
   const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
-  const int c = a.c, units = c / E;
+  const int c = a.c;
+  float pw[S::EPL], pb[S::EPL], sc[S::EPL], qw[S::EPL], qb[S::EPL];
+  if (a.f) {
+    rj_vector<S>(a.post_weight, 1.f, 1.f, lane, c, pw);
+    rj_vector<S>(a.post_bias, 0.f, 1.f, lane, c, pb);
+    rj_vector<S>(a.scale, 1.f, a.alpha, lane, c, sc);
+  }
+  if (a.pre_kind) {
+    rj_vector<S>(a.pre_weight, 1.f, 1.f, lane, c, qw);
+    rj_vector<S>(a.pre_bias, 0.f, 1.f, lane, c, qb);
+  }
   for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
-    const int64_t row = base + sub < a.n ? base + sub : a.n - 1;
     const bool mine = base + sub < a.n;
-    float h[S::EPL];
+    const int64_t row = mine ? base + sub : a.n - 1;
+    typename Row::Raw rx[NV], rf[NV], rg[NV];
+    float ag = 1.f, dag;
+    // every load of the row first
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int unit = k * T + lane;
-#pragma unroll
-      for (int j = 0; j < E; ++j) h[k * E + j] = 0.f;
-      if (unit < units) A8Row<BF16, E>::load(a.x, row * a.x_stride + unit * E, h + k * E);
+      const int at = (k * T + lane) * E;
+      const bool in = at < c;
+      rx[k] = in ? Row::fetch((const char *)a.x + row * a.x_stride * (S::BF16 ? 2 : 4), at) : Row::zero();
+      if (a.f) rf[k] = in ? Row::fetch((const char *)a.f + row * a.f_stride * (S::BF16 ? 2 : 4), at) : Row::zero();
+      if (a.gate_cols > 1) rg[k] = in ? Row::fetch((const char *)a.gate + row * a.gate_stride * (S::BF16 ? 2 : 4), at) : Row::zero();
     }
+    if (a.gate_cols == 1) A8Row<S::BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
+    float h[S::EPL];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) Row::unpack(rx[k], h + k * E);
     if (a.x_codes) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -119,12 +161,7 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
     if (a.f) {
       float f[S::EPL];
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int unit = k * T + lane;
-#pragma unroll
-        for (int j = 0; j < E; ++j) f[k * E + j] = 0.f;
-        if (unit < units) A8Row<BF16, E>::load(a.f, row * a.f_stride + unit * E, f + k * E);
-      }
+      for (int k = 0; k < NV; ++k) Row::unpack(rf[k], f + k * E);
       if (a.f_codes) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -133,49 +170,41 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
         }
       }
       float r = 1.f;
-      if (a.post_kind) r = rj_normalise<T, S::NT, E, NV>(a.post_kind, a.post_eps, p.inv_c, lane, units, f, lds1, slot);
-      float ag = 1.f, dag;
-      if (a.gate_cols == 1) {
-        A8Row<BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
-        rj_act(a.gate_act, ag, ag, dag);
-      }
+      if (a.post_kind) r = rj_normalise<S>(a.post_kind, a.post_eps, p.inv_c, lane, c, f, lds1, slot);
+      if (a.gate_cols == 1 && a.gate_act != D3D_GATE_NONE) rj_act<false>(a.gate_act, ag, ag, dag);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int at = (k * T + lane) * E;
-        if (at >= c) continue;
-        float gt[E];
-        if (a.gate_cols > 1) A8Row<BF16, E>::load(a.gate, row * a.gate_stride + at, gt);
+        float g[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) g[j] = ag;
+        if (a.gate_cols > 1) {
+          Row::unpack(rg[k], g);
+          if (a.gate_act != D3D_GATE_NONE) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) rj_act<false>(a.gate_act, g[j], g[j], dag);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          float u = f[k * E + j] * r;
-          if (a.post_weight) u *= a.post_weight[at + j];
-          if (a.post_bias) u += a.post_bias[at + j];
-          float m = a.alpha * ag;
-          if (a.scale) m *= a.scale[at + j];
-          if (a.gate_cols > 1) {
-            float av;
-            rj_act(a.gate_act, gt[j], av, dag);
-            m *= av;
-          }
-          h[k * E + j] = fmaf(m, u, h[k * E + j]);
+          const int q = k * E + j;
+          h[q] = fmaf(sc[q] * g[j], fmaf(f[q] * r, pw[q], pb[q]), h[q]);
         }
-        if (a.h && mine) A8Row<BF16, E>::store(a.h, row * (int64_t)c + at, h + k * E);
+        const int at = (k * T + lane) * E;
+        if (mine && at < c) Row::store(a.h, row * (int64_t)c + at, h + k * E);
+        if (at >= c) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) h[k * E + j] = 0.f;
+        }
       }
     }
     if (a.pre_kind) {
-      const float r = rj_normalise<T, S::NT, E, NV>(a.pre_kind, a.pre_eps, p.inv_c, lane, units, h, lds1, slot);
+      const float r = rj_normalise<S>(a.pre_kind, a.pre_eps, p.inv_c, lane, c, h, lds1, slot);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int at = (k * T + lane) * E;
-        if (at >= c) continue;
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          float z = h[k * E + j] * r;
-          if (a.pre_weight) z *= a.pre_weight[at + j];
-          if (a.pre_bias) z += a.pre_bias[at + j];
-          h[k * E + j] = z;
-        }
-        if (mine) A8Row<BF16, E>::store(a.z, row * (int64_t)c + at, h + k * E);
+        for (int j = 0; j < E; ++j) h[k * E + j] = fmaf(h[k * E + j] * r, qw[k * E + j], qb[k * E + j]);
+        if (mine && at < c) Row::store(a.z, row * (int64_t)c + at, h + k * E);
       }
     }
   }
@@ -213,104 +242,123 @@ __device__ __forceinline__ void rj_columns(const float *acc, int c, float *lds, 
 
 // HELD: 0 rows as they are, 1 + format: codes
 template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_bwd_kernel(RjArgs p) {
-  constexpr bool BF16 = S::BF16;
-  constexpr int E = S::E, T = S::T, NV = S::NV;
+  constexpr int E = S::E, T = S::T, NV = S::NV, EB = S::BF16 ? 2 : 4;
   constexpr int FMT = HELD == 2 ? D3D_ACT8_E4M3 : D3D_ACT8_INT8;
-  constexpr int GL = A8_GROUP / E < T ? A8_GROUP / E : T;
+  using Row = A8Row<S::BF16, E>;
+  using Code = A8Held<FMT, E, 1>;
+  using In = typename std::conditional<HELD != 0, Code, Row>::type;  // what x and f come as
   __shared__ float lds1[2][1][S::NT / 64], lds2[2][2][S::NT / 64], lds3[2][3][S::NT / 64];
   __shared__ float cols[S::RPB > 1 ? S::NT * S::EPL : 1];
   int slot1 = 0, slot2 = 0, slot3 = 0;
   const D3dRowJoin &a = p.a;
   const D3dRowJoinGrads &g = p.g;
   const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
-  const int c = a.c, units = c / E;
+  const int c = a.c;
   const bool has_f = HELD ? a.f_codes != nullptr : a.f != nullptr;
+  float pw[S::EPL], pb[S::EPL], sc[S::EPL], qw[S::EPL];
+  if (has_f) {
+    rj_vector<S>(a.post_weight, 1.f, 1.f, lane, c, pw);
+    rj_vector<S>(a.post_bias, 0.f, 1.f, lane, c, pb);
+    rj_vector<S>(a.scale, 1.f, a.alpha, lane, c, sc);
+  }
+  if (a.pre_kind) rj_vector<S>(a.pre_weight, 1.f, 1.f, lane, c, qw);
   float s_scale[S::EPL], s_pw[S::EPL], s_pb[S::EPL], s_qw[S::EPL], s_qb[S::EPL];
 #pragma unroll
   for (int j = 0; j < S::EPL; ++j) s_scale[j] = s_pw[j] = s_pb[j] = s_qw[j] = s_qb[j] = 0.f;
 
   for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
-    const int64_t row = base + sub < a.n ? base + sub : a.n - 1;
     const bool mine = base + sub < a.n;
-    float h[S::EPL], f[S::EPL], m[S::EPL], dm[S::EPL];  // x, then h, then hhat | f, then fhat | factor of u | act'(g) alpha s
-    auto fetch = [&](const void *src, int64_t stride, const uint8_t *codes, const uint8_t *scales, float *v) {
+    const int64_t row = mine ? base + sub : a.n - 1;
+    // every load of the row first.  A row behind the last takes part in the sums over lanes with zero gradients, so that it
+    // adds nothing to the columns
+    typename In::Raw rx[NV], rf[NV];
+    typename Row::Raw rg[NV], rdh[NV], rdz[NV];
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int at = (k * T + lane) * E;
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[k * E + j] = 0.f;
-        if (at < c) {
-          if constexpr (HELD) A8Held<FMT, E, GL>::load(codes, scales, row, p.pitch, at, v + k * E);
-          else A8Row<BF16, E>::load(src, row * stride + at, v + k * E);
-        }
+    for (int k = 0; k < NV; ++k) {
+      const int at = (k * T + lane) * E;
+      const bool in = at < c;
+      if constexpr (HELD != 0) {
+        rx[k] = in ? Code::fetch(a.x_codes, a.x_scales, row, p.pitch, at) : Code::zero();
+        if (has_f) rf[k] = in ? Code::fetch(a.f_codes, a.f_scales, row, p.pitch, at) : Code::zero();
+      } else {
+        rx[k] = in ? Row::fetch((const char *)a.x + row * a.x_stride * EB, at) : Row::zero();
+        if (has_f) rf[k] = in ? Row::fetch((const char *)a.f + row * a.f_stride * EB, at) : Row::zero();
       }
-    };
-    fetch(a.x, a.x_stride, a.x_codes, a.x_scales, h);
-    float fr = 1.f, ag = 1.f, dag = 0.f;
+      rg[k] = in && a.gate_cols > 1 ? Row::fetch((const char *)a.gate + row * a.gate_stride * EB, at) : Row::zero();
+      rdz[k] = in && mine && g.dz ? Row::fetch((const char *)g.dz + row * g.dz_stride * EB, at) : Row::zero();
+      rdh[k] = in && mine && g.dh ? Row::fetch((const char *)g.dh + row * g.dh_stride * EB, at) : Row::zero();
+    }
+    float ag = 1.f, dag = 0.f;
+    if (a.gate_cols == 1) A8Row<S::BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
+
+    float h[S::EPL], f[S::EPL], m[S::EPL], dm[S::EPL];  // x, then h, then hhat | f, then fhat | act(g) | act'(g)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) In::unpack(rx[k], h + k * E);
+    float fr = 1.f;
     if (has_f) {
-      fetch(a.f, a.f_stride, a.f_codes, a.f_scales, f);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) In::unpack(rf[k], f + k * E);
       if (a.post_kind) {
-        fr = rj_normalise<T, S::NT, E, NV>(a.post_kind, a.post_eps, p.inv_c, lane, units, f, lds1, slot1);
+        fr = rj_normalise<S>(a.post_kind, a.post_eps, p.inv_c, lane, c, f, lds1, slot1);
 #pragma unroll
         for (int j = 0; j < S::EPL; ++j) f[j] *= fr;
       }
       if (a.gate_cols == 1) {
-        A8Row<BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
-        rj_act(a.gate_act, ag, ag, dag);
+        dag = 1.f;
+        if (a.gate_act != D3D_GATE_NONE) rj_act<true>(a.gate_act, ag, ag, dag);
       }
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int at = (k * T + lane) * E;
-        float gt[E];
-        if (at < c && a.gate_cols > 1) A8Row<BF16, E>::load(a.gate, row * a.gate_stride + at, gt);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          m[k * E + j] = ag;
+          dm[k * E + j] = 1.f;
+        }
+        if (a.gate_cols > 1) {
+          Row::unpack(rg[k], m + k * E);
+          if (a.gate_act != D3D_GATE_NONE) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) rj_act<true>(a.gate_act, m[k * E + j], m[k * E + j], dm[k * E + j]);
+          }
+        }
+        const bool in = (k * T + lane) * E < c;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const int q = k * E + j;
-          m[q] = dm[q] = 0.f;
-          if (at >= c) continue;
-          float av = ag, dv = dag;
-          if (a.gate_cols > 1) rj_act(a.gate_act, gt[j], av, dv);
-          m[q] = av;   // act(g)
-          dm[q] = dv;  // act'(g)
-          float u = f[q];
-          if (a.post_weight) u *= a.post_weight[at + j];
-          if (a.post_bias) u += a.post_bias[at + j];
-          const float s = a.scale ? a.alpha * a.scale[at + j] : a.alpha;
-          h[q] = fmaf(s * av, u, h[q]);
+          const float v = fmaf(sc[q] * m[q], fmaf(f[q], pw[q], pb[q]), h[q]);
+          h[q] = in ? v : 0.f;
         }
       }
     }
     float d[S::EPL];  // dH
-    float hr = 1.f;
     if (a.pre_kind) {
-      hr = rj_normalise<T, S::NT, E, NV>(a.pre_kind, a.pre_eps, p.inv_c, lane, units, h, lds1, slot1);
+      const float hr = rj_normalise<S>(a.pre_kind, a.pre_eps, p.inv_c, lane, c, h, lds1, slot1);
       float s2[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int at = (k * T + lane) * E;
         float dz[E];
-#pragma unroll
-        for (int j = 0; j < E; ++j) dz[j] = 0.f;
-        if (at < c && g.dz) A8Row<BF16, E>::load(g.dz, row * g.dz_stride + at, dz);
+        Row::unpack(rdz[k], dz);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const int q = k * E + j;
           h[q] *= hr;
-          d[q] = 0.f;
-          if (at >= c) continue;
-          d[q] = a.pre_weight ? dz[j] * a.pre_weight[at + j] : dz[j];
-          if (mine) {
+          d[q] = dz[j] * qw[q];
+          s2[0] = fmaf(d[q], h[q], s2[0]);
+          s2[1] += d[q];
+        }
+        if (mine) {  // (not 0 times a NaN of the last row)
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const int q = k * E + j;
             s_qw[q] = fmaf(dz[j], h[q], s_qw[q]);
             s_qb[q] += dz[j];
           }
-          s2[0] = fmaf(d[q], h[q], s2[0]);
-          s2[1] += d[q];
         }
       }
       row_sum<T, S::NT, 2>(s2, lds2, slot2);
       const float m2 = s2[0] * p.inv_c, m1 = a.pre_kind == D3D_NORM_LAYER ? s2[1] * p.inv_c : 0.f;
 #pragma unroll
-      for (int j = 0; j < S::EPL; ++j) d[j] = hr * (d[j] - m1 - h[j] * m2);
+      for (int j = 0; j < S::EPL; ++j) d[j] = hr * (fmaf(-h[j], m2, d[j]) - m1);
     } else {
 #pragma unroll
       for (int j = 0; j < S::EPL; ++j) d[j] = 0.f;
@@ -318,65 +366,55 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
-      if (at >= c) continue;
-      if (g.dh) {
-        float dh[E];
-        A8Row<BF16, E>::load(g.dh, row * g.dh_stride + at, dh);
+      float dh[E];
+      Row::unpack(rdh[k], dh);
+      const bool in = at < c;
 #pragma unroll
-        for (int j = 0; j < E; ++j) d[k * E + j] += dh[j];
-      }
-      if (g.dx && mine) A8Row<BF16, E>::store(g.dx, row * (int64_t)c + at, d + k * E);
+      for (int j = 0; j < E; ++j) d[k * E + j] = in ? d[k * E + j] + dh[j] : 0.f;
+      if (g.dx && mine && in) Row::store(g.dx, row * (int64_t)c + at, d + k * E);
     }
     if (!has_f) continue;
     float s3[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
-      if (at >= c) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) d[k * E + j] = 0.f;
-        continue;
-      }
       float dg[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int q = k * E + j;
-        float u = f[q];
-        if (a.post_weight) u *= a.post_weight[at + j];
-        if (a.post_bias) u += a.post_bias[at + j];
-        const float s = a.scale ? a.alpha * a.scale[at + j] : a.alpha;
-        dg[j] = d[q] * s * u;
-        const float du = d[q] * s * m[q];
+        const float u = fmaf(f[q], pw[q], pb[q]), e = d[q] * m[q], du = e * sc[q];
+        dg[j] = d[q] * sc[q] * u;
+        s3[2] += dg[j];
+        dg[j] *= dm[q];
         if (mine) {
-          s_scale[q] = fmaf(a.alpha * d[q] * m[q], u, s_scale[q]);
+          s_scale[q] = fmaf(e, u, s_scale[q]);
           s_pw[q] = fmaf(du, f[q], s_pw[q]);
           s_pb[q] += du;
         }
-        s3[2] += dg[j];
-        dg[j] *= dm[q];
-        d[q] = a.post_weight ? du * a.post_weight[at + j] : du;
+        d[q] = du * pw[q];
         s3[0] = fmaf(d[q], f[q], s3[0]);
         s3[1] += d[q];
       }
-      if (g.dgate && a.gate_cols > 1 && mine) A8Row<BF16, E>::store(g.dgate, row * (int64_t)c + at, dg);
+      if (g.dgate && a.gate_cols > 1 && mine && at < c) Row::store(g.dgate, row * (int64_t)c + at, dg);
     }
     row_sum<T, S::NT, 3>(s3, lds3, slot3);
     if (g.dgate && a.gate_cols == 1 && mine && lane == 0) {
       const float v = s3[2] * dag;
-      A8Row<BF16, 1>::store(g.dgate, row, &v);
+      A8Row<S::BF16, 1>::store(g.dgate, row, &v);
     }
     const float m2 = s3[0] * p.inv_c, m1 = a.post_kind == D3D_NORM_LAYER ? s3[1] * p.inv_c : 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
-      if (at >= c) continue;
       if (a.post_kind) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) d[k * E + j] = fr * (d[k * E + j] - m1 - f[k * E + j] * m2);
+        for (int j = 0; j < E; ++j) d[k * E + j] = fr * (fmaf(-f[k * E + j], m2, d[k * E + j]) - m1);
       }
-      if (g.df && mine) A8Row<BF16, E>::store(g.df, row * (int64_t)c + at, d + k * E);
+      if (g.df && mine && at < c) Row::store(g.df, row * (int64_t)c + at, d + k * E);
     }
   }
+#pragma unroll
+  for (int j = 0; j < S::EPL; ++j) s_scale[j] *= a.alpha;
   float *const results[5] = {g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
   const float *const accs[5] = {s_scale, s_pw, s_pb, s_qw, s_qb};
   int at = 0;
@@ -388,21 +426,37 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
   }
 }
 
-__global__ void __launch_bounds__(256) row_join_fold_kernel(const float *__restrict__ part, int blocks, int sums, int c, D3dRowJoinGrads g) {
+// the blocks' slabs added up: 32 columns a block, 32 parts of the slabs side by side, the parts in a tree.  (One thread a column
+// over all slabs took 117 us for 512 of them: as many dependent loads.)
+__global__ void __launch_bounds__(1024) row_join_fold_kernel(const float *__restrict__ part, int blocks, int sums, int c, D3dRowJoinGrads g) {
+  __shared__ float lds[32][33];
   float *const all[5] = {g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < sums * c; i += gridDim.x * 256) {
-    float t = 0.f;
-    for (int b = 0; b < blocks; ++b) t += part[(int64_t)b * sums * c + i];
-    int left = i / c;
-    for (int k = 0; k < 5; ++k)
-      if (all[k] && left-- == 0) all[k][i % c] = t;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + x;
+  const int64_t step = (int64_t)sums * c;
+  float t = 0.f;
+  if (i < sums * c) {
+#pragma unroll 4
+    for (int b = y; b < blocks; b += 32) t += part[b * step + i];
   }
+  lds[y][x] = t;
+  __syncthreads();
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    if (y < m) lds[y][x] += lds[y + m][x];
+    __syncthreads();
+  }
+  if (y != 0 || i >= sums * c) return;
+  int left = i / c;
+#pragma unroll
+  for (int k = 0; k < 5; ++k)
+    if (all[k] && left-- == 0) all[k][i % c] = lds[0][x];
 }
 
 #define RJ_MAXC 8192
-static int rj_blocks_bwd(int64_t n, int rpb) {
-  const int64_t nb = (n + rpb - 1) / rpb;
-  return (int)(nb < 1 ? 1 : (nb > 512 ? 512 : nb));
+static int rj_blocks_bwd(int64_t n, int rpb, int nt) {
+  const int64_t nb = (n + rpb - 1) / rpb, most = nt > 256 ? 512 : 1024;
+  return (int)(nb > most ? most : nb);
 }
 
 static int rj_check(const D3dRowJoin *a, bool backward, const char *who) {
@@ -428,11 +482,13 @@ static int rj_check(const D3dRowJoin *a, bool backward, const char *who) {
   D3D_REQUIRE((((uintptr_t)a->x_codes | (uintptr_t)a->f_codes) & 15) == 0, "%s: codes are not aligned to 16 bytes", who);
   return D3D_OK;
 }
-// may the rows be moved as 16-byte vectors?  (the float32 vectors over the channels are read value by value)
+// may the rows, and the float32 vectors over the channels, be moved 16 bytes at a time?
 static bool rj_vectors(const D3dRowJoin *a, const D3dRowJoinGrads *g) {
   const int eb = a->dtype == D3D_BF16 ? 2 : 4;
   bool v = a8_vectors(a->x, a->x_stride, a->c, eb) && a8_vectors(a->f, a->f_stride, a->c, eb) && a8_vectors(a->h, a->c, a->c, eb) &&
            a8_vectors(a->z, a->c, a->c, eb) && a->c % (16 / eb) == 0;
+  for (const void *w : {(const void *)a->scale, (const void *)a->post_weight, (const void *)a->post_bias, (const void *)a->pre_weight, (const void *)a->pre_bias})
+    v = v && ((uintptr_t)w & 15) == 0;
   if (a->gate_cols > 1) v = v && a8_vectors(a->gate, a->gate_stride, a->c, eb);
   if (g) {
     v = v && a8_vectors(g->dh, g->dh_stride, a->c, eb) && a8_vectors(g->dz, g->dz_stride, a->c, eb) &&
@@ -460,8 +516,10 @@ template <bool BF16, class Go> static int rj_pick(int c, bool vec, Go &&go) {
   }
   if (c <= 32) return go(RjShape<BF16, 1, 32, 1>{});
   if (c <= 64) return go(RjShape<BF16, 1, 64, 1>{});
+  if (c <= 128) return go(RjShape<BF16, 1, 64, 2>{});
   if (c <= 256) return go(RjShape<BF16, 1, 64, 4>{});
-  if (c <= 1024) return go(RjShape<BF16, 1, 256, 4>{});
+  if (c <= 512) return go(RjShape<BF16, 1, 64, 8>{});
+  if (c <= 2048) return go(RjShape<BF16, 1, 256, 8>{});
   return go(RjShape<BF16, 1, 1024, 8>{});
 }
 template <class Go> static int rj_for(const D3dRowJoin *a, bool vec, Go &&go) {
@@ -482,7 +540,9 @@ extern "C" int d3d_row_join_fwd(const D3dRowJoin *a, d3d_stream_t stream_) {
   rj_for(a, vec, [&](auto shape) {
     using S = decltype(shape);
     const int64_t nb = (a->n + S::RPB - 1) / S::RPB;
-    const dim3 grid((unsigned)(nb > 65536 ? 65536 : nb));
+    // (a block keeps the [c] vectors in registers from row to row: enough blocks to fill the chip, no more)
+    const int64_t most = 256 * (2048 / S::NT);
+    const dim3 grid((unsigned)(nb > most ? most : nb));
     if (a->fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((row_join_fwd_kernel<S, D3D_ACT8_INT8>), grid, dim3(S::NT), 0, stream, p);
     else hipLaunchKernelGGL((row_join_fwd_kernel<S, D3D_ACT8_E4M3>), grid, dim3(S::NT), 0, stream, p);
     return D3D_OK;
@@ -494,7 +554,7 @@ extern "C" int d3d_row_join_fwd(const D3dRowJoin *a, d3d_stream_t stream_) {
 // workspace of the column sums: an upper bound over the row layouts (rows per block), which depend on alignment too
 extern "C" size_t d3d_row_join_ws_floats(int64_t n, int c, int dtype, int sums) {
   if (n < 1 || c < 1 || c > RJ_MAXC || sums < 1 || sums > 5 || (dtype != D3D_F32 && dtype != D3D_BF16)) return 0;
-  return (size_t)rj_blocks_bwd(n, 1) * (size_t)sums * (size_t)c;
+  return (size_t)rj_blocks_bwd(n, 1, 256) * (size_t)sums * (size_t)c;
 }
 
 extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d3d_stream_t stream_) {
@@ -524,7 +584,7 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
   int blocks = 0;
   rc = rj_for(a, vec, [&](auto shape) {
     using S = decltype(shape);
-    blocks = rj_blocks_bwd(a->n, S::RPB);
+    blocks = rj_blocks_bwd(a->n, S::RPB, S::NT);
     if (sums && blocks > 1) {
       const size_t need = (size_t)blocks * sums * a->c;
       if (!g->ws || g->ws_floats < need)
@@ -540,8 +600,8 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
   if (rc) return rc;
   D3D_LAUNCH_TRY("row_join_bwd_kernel");
   if (p.part) {
-    const int nb = (sums * a->c + 255) / 256;
-    hipLaunchKernelGGL(row_join_fold_kernel, dim3(nb), dim3(256), 0, stream, p.part, blocks, sums, a->c, *g);
+    const int nb = (sums * a->c + 31) / 32;
+    hipLaunchKernelGGL(row_join_fold_kernel, dim3(nb), dim3(1024), 0, stream, p.part, blocks, sums, a->c, *g);
     D3D_LAUNCH_TRY("row_join_fold_kernel");
   }
   return D3D_OK;

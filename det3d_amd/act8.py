@@ -148,7 +148,7 @@ def weight_grad(held, dy, nbr=None):
     Entries of the table outside [0, n_in) are absent neighbours and add nothing.  Products are exact to float32 (bfloat16 `dy`: as
     they are; float32 `dy`: in three bfloat16 terms), sums are float32 in a fixed order.  Non-finite values in `dy` make the
     columns that they reach NaN."""
-    dy = rows_of(dy.detach(), "act8.weight_grad")
+    dy = rows_of(dy, "act8.weight_grad")
     n_in, cin = held.shape
     n_out, cout = dy.shape
     dev = dy.device

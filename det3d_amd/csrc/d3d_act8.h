@@ -58,6 +58,14 @@ template <int FMT> __device__ __forceinline__ void a8_value4(uint32_t w, float u
   }
 }
 
+// 4, 8 or 16 bytes at any address: one load / store on gfx950 (unaligned access mode), the same as an aligned one
+template <class V> __device__ __forceinline__ V a8_get(const void *p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+template <class V> __device__ __forceinline__ void a8_put(void *p, const V &v) { __builtin_memcpy(p, &v, sizeof(V)); }
+
 typedef __attribute__((ext_vector_type(2))) float a8_f32x2;
 typedef __attribute__((ext_vector_type(2))) __bf16 a8_bf16x2;
 __device__ __forceinline__ uint32_t a8_pack_bf16(float a, float b) {  // round to nearest even

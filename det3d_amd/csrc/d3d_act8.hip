@@ -113,7 +113,7 @@ extern "C" int d3d_act8_restore(const uint8_t *codes, const uint8_t *scales, int
 //   * dy's chunk goes through LDS once, as P bf16 planes (f32: three, hi + mid + lo = all 24 bits; restored values are exact in
 //     bf16, so the products are exact to f32 either way), and stays in registers as the MFMA's B operand for all KG units;
 //   * a unit's 64 x 64 codes are one 8-byte gather a thread, requested a whole chunk (KG units) ahead, its table entry a chunk
-//     further; restored to bf16 on the way into LDS (double buffered, one barrier a unit);
+//     further; restored to bf16 on the way into LDS (UB units at a time, double buffered, one barrier each);
 //   * both operands become MFMA fragments, rows as k, through the transposing read ds_read_b64_tr_b16.
 // Wave (wci, wco, wk): 32 of the unit's columns, 32 NB of dy's, every WK-th part of the chunk's rows; the wk parts are added in
 // the block, the row ranges through the workspace in their order.
@@ -131,7 +131,7 @@ struct Wg8Args {
   float *out;  // [splits][kvol][cin][cout], or dw itself
   int64_t dy_stride, cap, count;
   uint32_t n_in;
-  int n_out, cin, cinp, pitch, cout, cols, units, groups, cotiles, chunks, per_split, vec;
+  int n_out, cin, cinp, pitch, cout, cols, units, groups, cotiles, chunks, per_split;
 };
 
 template <int FMT> __device__ __forceinline__ uint4 wg8_restore(uint2 w, uint32_t b) {
@@ -181,15 +181,15 @@ template <int W> __device__ __forceinline__ a8_bf16x8 wg8_fragment(const unsigne
   return __builtin_bit_cast(a8_bf16x8, v);
 }
 
-template <int FMT, int P, int WCO, int WK, int NB, int KG, bool TABLE>
+template <int FMT, int P, int WCO, int WK, int NB, int KG, int UB, bool TABLE>
 __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   constexpr int TN = WCO * NB * 32, KS = WG8_ROWS / WK / 16;
   constexpr int VPT = TN >= 64 ? TN / 64 : 1;  // vectors of 8 columns of dy a thread stages
   constexpr int ABYTES = WG8_ROWS * 128, DBYTES = WG8_ROWS * TN * 2;
   constexpr int RBYTES = (WK - 1) * 2 * WCO * 4096;
-  constexpr int SMEM = 2 * ABYTES + P * DBYTES > RBYTES ? 2 * ABYTES + P * DBYTES : RBYTES;
+  constexpr int SMEM = 2 * UB * ABYTES + P * DBYTES > RBYTES ? 2 * UB * ABYTES + P * DBYTES : RBYTES;
   __shared__ __attribute__((aligned(16))) unsigned char smem[SMEM];
-  unsigned char *const sa = smem, *const sd = smem + 2 * ABYTES;
+  unsigned char *const sa = smem, *const sd = smem + 2 * UB * ABYTES;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -208,75 +208,79 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
 
   // this thread's 8 columns of each unit, and its row of the chunk
   const int srow = tid >> 3, sseg = tid & 7;
-  int ci[KG], tab[KG];  // column within the row of codes (-1: behind the last column) | offset k
+  int ci[KG];  // column within the row of codes (-1: behind the last column)
+  const int32_t *tab[TABLE ? KG : 1];  // its offset's entries
 #pragma unroll
   for (int u = 0; u < KG; ++u) {
     const int col = (unit0 + u) * 64 + sseg * 8;
     const bool in = u < nu && col < p.cols;
-    tab[u] = TABLE && in ? col / p.cinp : 0;
-    ci[u] = in ? col - tab[u] * p.cinp : -1;
+    const int k = TABLE && in ? col / p.cinp : 0;
+    ci[u] = in ? col - k * p.cinp : -1;
+    if constexpr (TABLE) tab[u] = p.nbr + k * p.cap;
   }
   int32_t idx[KG];
   uint2 code[KG];
   uint32_t sc[KG];
-  auto load_idx = [&](int u, int chunk) {  // rows behind the last and columns behind the last: absent
-    const int o = (chunk0 + chunk) * WG8_ROWS + srow;
-    idx[u] = -1;
-    if (chunk < chunks && o < p.n_out && ci[u] >= 0) idx[u] = TABLE ? p.nbr[tab[u] * p.cap + o] : o;
+  // Loads stay in flight only while nothing touches their registers: no select behind them, no branch that two of them share.
+  // What is absent reads beyond the buffer and gets zeros (a scale of 0: the row adds nothing).  Table entries and codes lie
+  // within 2^31 bytes of their bases (checked on the host); without a table the base moves with the chunk.
+  auto there = [&](int u, int chunk) -> bool {
+    return (chunk < chunks) & ((chunk0 + chunk) * WG8_ROWS + srow < p.n_out) & (ci[u] >= 0);
   };
-  auto load_code = [&](int u) {
-    const bool in = (uint32_t)idx[u] < p.n_in;
-    const int64_t row = in ? idx[u] : 0;
-    const int c = in ? ci[u] : 0;
-    code[u] = *(const uint2 *)(p.codes + row * p.pitch + c);
-    const uint32_t b = p.scales[row * (p.pitch >> 5) + (c >> 5)];
-    sc[u] = in ? b : 0u;  // scale 0: the row adds nothing
+  auto load_idx = [&](int u, int chunk) {
+    if constexpr (TABLE) idx[u] = tab[u][there(u, chunk) ? (chunk0 + chunk) * WG8_ROWS + srow : 0];
   };
+  auto load_code = [&](int u, int chunk) {
+    const uint32_t row = TABLE ? (uint32_t)idx[u] : (uint32_t)srow;
+    const bool in = there(u, chunk) & (!TABLE | (row < p.n_in));
+    const uint32_t off = row * (uint32_t)p.pitch + (uint32_t)ci[u];
+    const int64_t base = TABLE ? 0 : (int64_t)(chunk0 + chunk) * WG8_ROWS * p.pitch;
+    code[u] = d3d_buffer_load8(d3d_make_rsrc(p.codes + base), in ? off : D3D_OOB_OFFSET);
+    sc[u] = __builtin_amdgcn_raw_buffer_load_b8(d3d_make_rsrc(p.scales + (base >> 5)), (int)(in ? off >> 5 : D3D_OOB_OFFSET), 0, 0);
+  };  // (a row of codes is a whole number of groups: group = off / 32)
 
-  // dy: thread's vectors of the chunk
-  float dyv[P == 3 ? VPT * 8 : 1];
-  uint4 dyb[P == 3 ? 1 : VPT];
+  // dy: this thread's vectors of 8 columns of the chunk, as they come; rows behind the last read the last one and are zeroed
+  // where they are unpacked, columns behind the last are zeroed here (in the few waves that have them)
+  constexpr int DW = P == 3 ? 8 : 4, EB = P == 3 ? 4 : 2;  // words of a vector, bytes of a value
+  uint32_t dyr[VPT][DW];
   auto load_dy = [&](int chunk) {
+    const int last = p.n_out - 1 - (chunk0 + chunk) * WG8_ROWS;
+    const char *base = (const char *)p.dy + (int64_t)(chunk0 + chunk) * WG8_ROWS * p.dy_stride * EB;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int i = tid + 512 * v, r = i / (TN / 8), cv = i % (TN / 8);
-      const int o = (chunk0 + chunk) * WG8_ROWS + r, co = co0 + cv * 8;
-      const bool in = r < WG8_ROWS && o < p.n_out && co < p.cout;
-      if constexpr (P == 3) {
-        const float *src = (const float *)p.dy + (int64_t)(in ? o : 0) * p.dy_stride;
-        if (p.vec && co + 8 <= p.cout) {
-          const float4 x = in ? *(const float4 *)(src + co) : make_float4(0, 0, 0, 0);
-          const float4 y = in ? *(const float4 *)(src + co + 4) : make_float4(0, 0, 0, 0);
-          dyv[v * 8] = x.x; dyv[v * 8 + 1] = x.y; dyv[v * 8 + 2] = x.z; dyv[v * 8 + 3] = x.w;
-          dyv[v * 8 + 4] = y.x; dyv[v * 8 + 5] = y.y; dyv[v * 8 + 6] = y.z; dyv[v * 8 + 7] = y.w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dyv[v * 8 + j] = in && co + j < p.cout ? src[co + j] : 0.f;
+      const int i = tid + 512 * v, r = i / (TN / 8), co = co0 + i % (TN / 8) * 8;
+      const char *src = base + ((int64_t)(r < last ? r : last) * p.dy_stride + co) * EB;
+      if (co + 8 <= p.cout) {
+        const uint4 x = a8_get<uint4>(src);
+        dyr[v][0] = x.x; dyr[v][1] = x.y; dyr[v][2] = x.z; dyr[v][3] = x.w;
+        if constexpr (P == 3) {
+          const uint4 y = a8_get<uint4>(src + 16);
+          dyr[v][4] = y.x; dyr[v][5] = y.y; dyr[v][6] = y.z; dyr[v][7] = y.w;
         }
       } else {
-        const uint16_t *src = (const uint16_t *)p.dy + (int64_t)(in ? o : 0) * p.dy_stride;
-        if (p.vec && co + 8 <= p.cout) {
-          dyb[v] = in ? *(const uint4 *)(src + co) : make_uint4(0, 0, 0, 0);
-        } else {
-          uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = in && co + j < p.cout ? src[co + j] : 0u;
-          dyb[v] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        for (int j = 0; j < DW; ++j) dyr[v][j] = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (co + j >= p.cout) continue;
+          if constexpr (P == 3) dyr[v][j] = *(const uint32_t *)(src + 4 * j);
+          else dyr[v][j / 2] |= (uint32_t)*(const uint16_t *)(src + 2 * j) << (j % 2 * 16);
         }
       }
     }
   };
-  auto write_dy = [&]() {
+  auto write_dy = [&](int chunk) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = tid + 512 * v, r = i / (TN / 8), cv = i % (TN / 8);
       if (r >= WG8_ROWS) continue;
+      const bool in = (chunk0 + chunk) * WG8_ROWS + r < p.n_out;
       const uint32_t at = wg8_slot<TN>(r, cv);
+      uint32_t w[P][4];
       if constexpr (P == 3) {
-        uint32_t w[3][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float a = dyv[v * 8 + 2 * j], b = dyv[v * 8 + 2 * j + 1];
+          float a = in ? __uint_as_float(dyr[v][2 * j]) : 0.f, b = in ? __uint_as_float(dyr[v][2 * j + 1]) : 0.f;
 #pragma unroll
           for (int q = 0; q < 3; ++q) {  // bf16 of what is left, and what that leaves (exact)
             w[q][j] = a8_pack_bf16(a, b);
@@ -284,11 +288,12 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
             b -= __uint_as_float(w[q][j] & 0xffff0000u);
           }
         }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *(uint4 *)(sd + q * DBYTES + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
       } else {
-        *(uint4 *)(sd + at) = dyb[v];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[0][j] = in ? dyr[v][j] : 0u;
       }
+#pragma unroll
+      for (int q = 0; q < P; ++q) *(uint4 *)(sd + q * DBYTES + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
     }
   };
 
@@ -305,17 +310,18 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   load_dy(0);
 #pragma unroll
   for (int u = 0; u < KG; ++u) {
-    load_code(u);
+    load_code(u, 0);
     load_idx(u, 1);
   }
   for (int chunk = 0; chunk < chunks; ++chunk) {
     auto stage = [&](int u) {
-      *(uint4 *)(sa + (u & 1) * ABYTES + wg8_slot<64>(srow, sseg)) = wg8_restore<FMT>(code[u], sc[u]);
-      load_code(u);  // of the next chunk (its index arrived a chunk ago)
+      *(uint4 *)(sa + (u % (2 * UB)) * ABYTES + wg8_slot<64>(srow, sseg)) = wg8_restore<FMT>(code[u], sc[u]);
+      load_code(u, chunk + 1);  // (its index arrived a chunk ago)
       load_idx(u, chunk + 2);
     };
-    write_dy();
-    stage(0);
+    write_dy(chunk);
+#pragma unroll
+    for (int u = 0; u < UB; ++u) stage(u);
     d3d_lds_barrier();
     a8_bf16x8 bf[KS][NB][P];
 #pragma unroll
@@ -324,22 +330,25 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int q = 0; q < P; ++q) bf[k][n][q] = wg8_fragment<TN>(sd + q * DBYTES, (wk * KS + k) * 16, (wco * NB + n) * 32);
-    if (chunk + 1 < chunks) load_dy(chunk + 1);
+    load_dy(chunk + 1 < chunks ? chunk + 1 : chunk);
+    // (units behind the last are worked on too, with zeros: a branch around them would make every wait for a load a wait for all)
 #pragma unroll
-    for (int u = 0; u < KG; ++u) {
-      if (u < nu) {
-        if (u + 1 < KG && u + 1 < nu) stage(u + 1);
+    for (int u0 = 0; u0 < KG; u0 += UB) {
+#pragma unroll
+      for (int u = u0 + UB; u < u0 + 2 * UB && u < KG; ++u) stage(u);
+#pragma unroll
+      for (int u = u0; u < u0 + UB; ++u) {
         a8_bf16x8 af[KS];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) af[k] = wg8_fragment<64>(sa + (u & 1) * ABYTES, (wk * KS + k) * 16, wci * 32);
+        for (int k = 0; k < KS; ++k) af[k] = wg8_fragment<64>(sa + (u % (2 * UB)) * ABYTES, (wk * KS + k) * 16, wci * 32);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int q = P - 1; q >= 0; --q) acc[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[k], bf[k][n][q], acc[u][n], 0, 0, 0);
-        d3d_lds_barrier();
       }
+      d3d_lds_barrier();
     }
   }
 
@@ -367,10 +376,13 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       }
       const int co = co0 + (wco * NB + n) * 32 + (lane & 31);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int col = (unit0 + u) * 64 + wci * 32 + (r >> 2) * 8 + ((lane >> 5) << 2) + (r & 3);
+      for (int r4 = 0; r4 < 4; ++r4) {  // four neighbouring columns of one offset
+        const int col = (unit0 + u) * 64 + wci * 32 + r4 * 8 + ((lane >> 5) << 2);
         const int k = col / p.cinp, c = col - k * p.cinp;
-        if (col < p.cols && c < p.cin && co < p.cout) p.out[split * p.count + ((int64_t)k * p.cin + c) * p.cout + co] = acc[u][n][r];
+        float *dst = p.out + split * p.count + ((int64_t)k * p.cin + c) * p.cout + co;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (col < p.cols && c + r < p.cin && co < p.cout) dst[(int64_t)r * p.cout] = acc[u][n][r4 * 4 + r];
       }
     }
   }
@@ -393,14 +405,15 @@ __global__ void __launch_bounds__(256) a8_fold_kernel(const float *__restrict__ 
 
 // how a weight gradient is cut: columns of dy a block, units, row ranges
 struct Wg8Plan {
-  int tn, units, groups, cotiles, chunks, per_split, splits;
+  int tn, kg, units, groups, cotiles, chunks, per_split, splits;
 };
-#define WG8_KG 4
+#define WG8_UB 2
 static Wg8Plan wg8_plan(int64_t n_out, int kvol, int cin, int cout, int dtype) {
   Wg8Plan q;
   q.tn = cout <= 32 ? 32 : (cout <= 64 ? 64 : (cout <= 128 || dtype == D3D_F32 ? 128 : 256));
   q.units = (int)(((int64_t)kvol * ((cin + 7) / 8 * 8) + 63) / 64);
-  q.groups = (q.units + WG8_KG - 1) / WG8_KG;
+  q.kg = q.units <= 2 ? 2 : 4;
+  q.groups = (q.units + q.kg - 1) / q.kg;
   q.cotiles = (cout + q.tn - 1) / q.tn;
   q.chunks = (int)((n_out + WG8_ROWS - 1) / WG8_ROWS);
   const int64_t tiles = (int64_t)q.groups * q.cotiles;
@@ -432,6 +445,8 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   D3D_REQUIRE(dy_stride >= cout, "d3d_act8_wgrad: rows of %d channels %lld elements apart", cout, (long long)dy_stride);
   D3D_REQUIRE(nbr ? cap >= n_out : (kvol == 1 && n_in == n_out), "d3d_act8_wgrad: cap=%lld kvol=%d n_in=%lld n_out=%lld",
               (long long)cap, kvol, (long long)n_in, (long long)n_out);
+  D3D_REQUIRE(!nbr || n_in * a8_pitch(cin) < ((int64_t)1 << 31), "d3d_act8_wgrad: %lld held rows of %d channels behind a table take 2 GB or more",
+              (long long)n_in, cin);
   const size_t need = d3d_act8_wgrad_workspace_bytes(n_out, kvol, cin, cout, dtype);
   if (need && (!workspace || workspace_bytes < need))
     return d3d_set_error(D3D_ECAPACITY, "d3d_act8_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -457,12 +472,13 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   p.cotiles = q.cotiles;
   p.chunks = q.chunks;
   p.per_split = q.per_split;
-  p.vec = ((uintptr_t)dy & 15) == 0 && dy_stride % (dtype == D3D_BF16 ? 8 : 4) == 0;
   const dim3 grid((unsigned)(q.groups * q.cotiles * q.splits));
 #define A8_WG(F, P, WCO, WK, NB)                                                                                                \
   do {                                                                                                                          \
-    if (nbr) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, WG8_KG, true>), grid, dim3(512), 0, stream, p);             \
-    else hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, WG8_KG, false>), grid, dim3(512), 0, stream, p);                \
+    if (nbr && q.kg == 2) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 2, WG8_UB, true>), grid, dim3(512), 0, stream, p);  \
+    else if (nbr) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 4, WG8_UB, true>), grid, dim3(512), 0, stream, p);     \
+    else if (q.kg == 2) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 2, WG8_UB, false>), grid, dim3(512), 0, stream, p); \
+    else hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 4, WG8_UB, false>), grid, dim3(512), 0, stream, p);             \
   } while (0)
 #define A8_WG_TN(F)                                                                                                             \
   do {                                                                                                                          \

@@ -130,32 +130,33 @@ struct Wg8Args {
   const int32_t *nbr;
   float *out;  // [splits][kvol][cin][cout], or dw itself
   int64_t dy_stride, cap, count;
-  uint32_t n_in;
+  uint32_t n_in, tab_bytes;
   int n_out, cin, cinp, pitch, cout, cols, units, groups, cotiles, chunks, per_split;
 };
 
 template <int FMT> __device__ __forceinline__ uint4 wg8_restore(uint2 w, uint32_t b) {
-  // 8 codes to bf16: exact, so the upper halves of the f32 values are taken as they are
+  // 8 codes to bf16: exact
   const float s = a8_up(b);
-  uint32_t v[8];
   if constexpr (FMT == D3D_ACT8_INT8) {
-    // biased to unsigned bytes, whose conversion is one instruction: (code + 128) 2^s - 128 2^s
+    // biased to unsigned bytes, whose conversion is one instruction: (code + 128) 2^s - 128 2^s; the upper halves of the f32
+    // values are their bf16
     const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
     const float m = -128.f * s;
+    uint32_t v[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[j] = __float_as_uint(fmaf((float)((x >> (8 * j)) & 0xffu), s, m));
       v[4 + j] = __float_as_uint(fmaf((float)((y >> (8 * j)) & 0xffu), s, m));
     }
+    return make_uint4(__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u),
+                      __builtin_amdgcn_perm(v[5], v[4], 0x07060302u), __builtin_amdgcn_perm(v[7], v[6], 0x07060302u));
   } else {
-    float f[8];
-    a8_value4<FMT>(w.x, s, f);
-    a8_value4<FMT>(w.y, s, f + 4);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(f[j]);
+    // two codes and the scale's exponent to a pair of bf16 in one instruction
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w.x, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w.x, s, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w.y, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w.y, s, true)));
   }
-  return make_uint4(__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u),
-                    __builtin_amdgcn_perm(v[5], v[4], 0x07060302u), __builtin_amdgcn_perm(v[7], v[6], 0x07060302u));
 }
 
 // byte of 16-byte slot `slot` in row r of a [rows][W columns] bf16 tile.  The slots of a row are permuted so that the four rows
@@ -181,7 +182,7 @@ template <int W> __device__ __forceinline__ a8_bf16x8 wg8_fragment(const unsigne
   return __builtin_bit_cast(a8_bf16x8, v);
 }
 
-template <int FMT, int P, int WCO, int WK, int NB, int KG, int UB, bool TABLE>
+template <int FMT, int P, int WCO, int WK, int NB, int KG, int UB, bool TABLE, bool EDGE>
 __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   constexpr int TN = WCO * NB * 32, KS = WG8_ROWS / WK / 16;
   constexpr int VPT = TN >= 64 ? TN / 64 : 1;  // vectors of 8 columns of dy a thread stages
@@ -206,81 +207,96 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   const int chunk0 = split * p.per_split;
   const int chunks = p.chunks - chunk0 < p.per_split ? p.chunks - chunk0 : p.per_split;
 
-  // this thread's 8 columns of each unit, and its row of the chunk
+  // Staging.  A thread owns one row of the chunk and 8 columns of each unit.  Loads stay in flight only while nothing touches
+  // their registers: no select behind them, no branch around them.  What is absent (a row or a column behind the last, a table
+  // entry out of range) reads beyond the buffer, which gives zeros: the scale 0 makes the row add nothing, whatever dy has there.
+  // Offsets are 32 bits: the table and the codes behind one stay below 2^31 bytes and 2^24 rows (checked on the host); without a
+  // table the base moves with the chunk.
   const int srow = tid >> 3, sseg = tid & 7;
-  int ci[KG];  // column within the row of codes (-1: behind the last column)
-  const int32_t *tab[TABLE ? KG : 1];  // its offset's entries
+  const int rows_here = p.n_out - chunk0 * WG8_ROWS;  // from the block's first row to the last
+  const int my_chunks = srow < rows_here ? min((rows_here - srow + WG8_ROWS - 1) / WG8_ROWS, chunks) : 0;
+  uint32_t col_off[KG], tab_off[TABLE ? KG : 1];
+  int lim[KG];  // chunks in which this thread has something of the unit
 #pragma unroll
   for (int u = 0; u < KG; ++u) {
     const int col = (unit0 + u) * 64 + sseg * 8;
     const bool in = u < nu && col < p.cols;
-    const int k = TABLE && in ? col / p.cinp : 0;
-    ci[u] = in ? col - k * p.cinp : -1;
-    if constexpr (TABLE) tab[u] = p.nbr + k * p.cap;
+    const int k = TABLE && in ? col / p.cinp : 0, ci = in ? col - k * p.cinp : 0;
+    lim[u] = in ? my_chunks : 0;
+    col_off[u] = TABLE ? (uint32_t)ci : (uint32_t)(srow * p.pitch + ci);
+    if constexpr (TABLE) tab_off[u] = ((uint32_t)k * (uint32_t)p.cap + (uint32_t)(chunk0 * WG8_ROWS + srow)) * 4u;
   }
-  int32_t idx[KG];
+  int32_t idx[TABLE ? KG : 1];
   uint2 code[KG];
   uint32_t sc[KG];
-  // Loads stay in flight only while nothing touches their registers: no select behind them, no branch that two of them share.
-  // What is absent reads beyond the buffer and gets zeros (a scale of 0: the row adds nothing).  Table entries and codes lie
-  // within 2^31 bytes of their bases (checked on the host); without a table the base moves with the chunk.
-  auto there = [&](int u, int chunk) -> bool {
-    return (chunk < chunks) & ((chunk0 + chunk) * WG8_ROWS + srow < p.n_out) & (ci[u] >= 0);
-  };
-  auto load_idx = [&](int u, int chunk) {
-    if constexpr (TABLE) idx[u] = tab[u][there(u, chunk) ? (chunk0 + chunk) * WG8_ROWS + srow : 0];
+  const __amdgpu_buffer_rsrc_t tab_rs = __builtin_amdgcn_make_buffer_rsrc((void *)p.nbr, 0, TABLE ? p.tab_bytes : 0, 0x00020000);
+  auto load_idx = [&](int u, int chunk) {  // (rows behind the last read other entries, or zeros: load_code knows)
+    if constexpr (TABLE) idx[u] = __builtin_amdgcn_raw_buffer_load_b32(tab_rs, (int)tab_off[u], chunk * (WG8_ROWS * 4), 0);
   };
   auto load_code = [&](int u, int chunk) {
-    const uint32_t row = TABLE ? (uint32_t)idx[u] : (uint32_t)srow;
-    const bool in = there(u, chunk) & (!TABLE | (row < p.n_in));
-    const uint32_t off = row * (uint32_t)p.pitch + (uint32_t)ci[u];
+    bool in = chunk < lim[u];
+    uint32_t off = col_off[u];
+    if constexpr (TABLE) {
+      in = in & ((uint32_t)idx[u] < p.n_in);
+      off += __umul24((uint32_t)idx[u], (uint32_t)p.pitch);
+    }
+    off = in ? off : D3D_OOB_OFFSET;
     const int64_t base = TABLE ? 0 : (int64_t)(chunk0 + chunk) * WG8_ROWS * p.pitch;
-    code[u] = d3d_buffer_load8(d3d_make_rsrc(p.codes + base), in ? off : D3D_OOB_OFFSET);
-    sc[u] = __builtin_amdgcn_raw_buffer_load_b8(d3d_make_rsrc(p.scales + (base >> 5)), (int)(in ? off >> 5 : D3D_OOB_OFFSET), 0, 0);
-  };  // (a row of codes is a whole number of groups: group = off / 32)
+    code[u] = d3d_buffer_load8(d3d_make_rsrc(p.codes + base), off);
+    // (a row of codes is a whole number of groups: group = off / 32; the absent offset / 32 lies behind 2^26 groups)
+    sc[u] = __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc((void *)(p.scales + (base >> 5)), 0, 1 << 26, 0x00020000), (int)(off >> 5), 0, 0);
+  };
 
-  // dy: this thread's vectors of 8 columns of the chunk, as they come; rows behind the last read the last one and are zeroed
-  // where they are unpacked, columns behind the last are zeroed here (in the few waves that have them)
-  constexpr int DW = P == 3 ? 8 : 4, EB = P == 3 ? 4 : 2;  // words of a vector, bytes of a value
+  // dy: this thread's vectors of 8 columns of the chunk, as they come; a row behind the last is the last one again (its partner
+  // in x is zero).  EDGE (the width is no multiple of 8): value by value, zeros behind the last column
+  constexpr int DW = P == 3 || EDGE ? 8 : 4, EB = P == 3 ? 4 : 2;  // words of a vector, bytes of a value
   uint32_t dyr[VPT][DW];
-  auto load_dy = [&](int chunk) {
-    const int last = p.n_out - 1 - (chunk0 + chunk) * WG8_ROWS;
-    const char *base = (const char *)p.dy + (int64_t)(chunk0 + chunk) * WG8_ROWS * p.dy_stride * EB;
+  const char *dyp[VPT];
+  int dy_chunk = 0;
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int i = tid + 512 * v, r = i / (TN / 8), co = co0 + i % (TN / 8) * 8;
+    const int row = r < rows_here ? r : rows_here - 1;
+    dyp[v] = (const char *)p.dy + ((int64_t)(chunk0 * WG8_ROWS + row) * p.dy_stride + (EDGE || co < p.cout ? co : 0)) * EB;
+  }
+  auto load_dy = [&]() {  // of the next chunk, as often as it is called
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int i = tid + 512 * v, r = i / (TN / 8), co = co0 + i % (TN / 8) * 8;
-      const char *src = base + ((int64_t)(r < last ? r : last) * p.dy_stride + co) * EB;
-      if (co + 8 <= p.cout) {
-        const uint4 x = a8_get<uint4>(src);
-        dyr[v][0] = x.x; dyr[v][1] = x.y; dyr[v][2] = x.z; dyr[v][3] = x.w;
-        if constexpr (P == 3) {
-          const uint4 y = a8_get<uint4>(src + 16);
-          dyr[v][4] = y.x; dyr[v][5] = y.y; dyr[v][6] = y.z; dyr[v][7] = y.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < DW; ++j) dyr[v][j] = 0u;
+      if constexpr (EDGE) {
+        const int co = co0 + (tid + 512 * v) % (TN / 8) * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (co + j >= p.cout) continue;
-          if constexpr (P == 3) dyr[v][j] = *(const uint32_t *)(src + 4 * j);
-          else dyr[v][j / 2] |= (uint32_t)*(const uint16_t *)(src + 2 * j) << (j % 2 * 16);
+          const char *src = dyp[v] + (co + j < p.cout ? j : p.cout - 1 - co) * EB;  // (columns behind the last: the last one)
+          if constexpr (P == 3) dyr[v][j] = *(const uint32_t *)src;
+          else dyr[v][j] = *(const uint16_t *)src;
+        }
+      } else {
+        const uint4 x = a8_get<uint4>(dyp[v]);
+        dyr[v][0] = x.x; dyr[v][1] = x.y; dyr[v][2] = x.z; dyr[v][3] = x.w;
+        if constexpr (P == 3) {
+          const uint4 y = a8_get<uint4>(dyp[v] + 16);
+          dyr[v][4] = y.x; dyr[v][5] = y.y; dyr[v][6] = y.z; dyr[v][7] = y.w;
         }
       }
     }
+    ++dy_chunk;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {  // on to the next row, while there is one
+      const int r = (tid + 512 * v) / (TN / 8);
+      if (dy_chunk * WG8_ROWS + r < rows_here) dyp[v] += (int64_t)WG8_ROWS * p.dy_stride * EB;
+    }
   };
-  auto write_dy = [&](int chunk) {
+  auto write_dy = [&]() {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = tid + 512 * v, r = i / (TN / 8), cv = i % (TN / 8);
-      if (r >= WG8_ROWS) continue;
-      const bool in = (chunk0 + chunk) * WG8_ROWS + r < p.n_out;
+      if (TN < 64 && r >= WG8_ROWS) continue;
       const uint32_t at = wg8_slot<TN>(r, cv);
       uint32_t w[P][4];
       if constexpr (P == 3) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float a = in ? __uint_as_float(dyr[v][2 * j]) : 0.f, b = in ? __uint_as_float(dyr[v][2 * j + 1]) : 0.f;
+          float a = __uint_as_float(dyr[v][2 * j]), b = __uint_as_float(dyr[v][2 * j + 1]);
 #pragma unroll
           for (int q = 0; q < 3; ++q) {  // bf16 of what is left, and what that leaves (exact)
             w[q][j] = a8_pack_bf16(a, b);
@@ -290,7 +306,10 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[0][j] = in ? dyr[v][j] : 0u;
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (EDGE) w[0][j] = dyr[v][2 * j] | dyr[v][2 * j + 1] << 16;
+          else w[0][j] = dyr[v][j];
+        }
       }
 #pragma unroll
       for (int q = 0; q < P; ++q) *(uint4 *)(sd + q * DBYTES + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
@@ -307,7 +326,8 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
 
 #pragma unroll
   for (int u = 0; u < KG; ++u) load_idx(u, 0);
-  load_dy(0);
+  load_dy();
+  __builtin_amdgcn_sched_barrier(0);  // (in this order, as in the loop: the waits at its top count the loads behind dy's)
 #pragma unroll
   for (int u = 0; u < KG; ++u) {
     load_code(u, 0);
@@ -319,7 +339,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       load_code(u, chunk + 1);  // (its index arrived a chunk ago)
       load_idx(u, chunk + 2);
     };
-    write_dy(chunk);
+    write_dy();
 #pragma unroll
     for (int u = 0; u < UB; ++u) stage(u);
     d3d_lds_barrier();
@@ -330,7 +350,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int q = 0; q < P; ++q) bf[k][n][q] = wg8_fragment<TN>(sd + q * DBYTES, (wk * KS + k) * 16, (wco * NB + n) * 32);
-    load_dy(chunk + 1 < chunks ? chunk + 1 : chunk);
+    load_dy();
     // (units behind the last are worked on too, with zeros: a branch around them would make every wait for a load a wait for all)
 #pragma unroll
     for (int u0 = 0; u0 < KG; u0 += UB) {
@@ -349,6 +369,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
             for (int q = P - 1; q >= 0; --q) acc[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[k], bf[k][n][q], acc[u][n], 0, 0, 0);
       }
       d3d_lds_barrier();
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -405,14 +426,15 @@ __global__ void __launch_bounds__(256) a8_fold_kernel(const float *__restrict__ 
 
 // how a weight gradient is cut: columns of dy a block, units, row ranges
 struct Wg8Plan {
-  int tn, kg, units, groups, cotiles, chunks, per_split, splits;
+  int tn, kg, edge, units, groups, cotiles, chunks, per_split, splits;
 };
 #define WG8_UB 2
-static Wg8Plan wg8_plan(int64_t n_out, int kvol, int cin, int cout, int dtype) {
+static Wg8Plan wg8_plan(int64_t n_out, int kvol, int cin, int cout, int dtype, bool table) {
   Wg8Plan q;
-  q.tn = cout <= 32 ? 32 : (cout <= 64 ? 64 : (cout <= 128 || dtype == D3D_F32 ? 128 : 256));
+  q.edge = cout % 8 != 0;
+  q.tn = cout <= 32 ? 32 : (cout <= 64 ? 64 : (cout <= 128 || dtype == D3D_F32 || q.edge ? 128 : 256));
   q.units = (int)(((int64_t)kvol * ((cin + 7) / 8 * 8) + 63) / 64);
-  q.kg = q.units <= 2 ? 2 : 4;
+  q.kg = q.units <= 2 && !table ? 2 : 4;
   q.groups = (q.units + q.kg - 1) / q.kg;
   q.cotiles = (cout + q.tn - 1) / q.tn;
   q.chunks = (int)((n_out + WG8_ROWS - 1) / WG8_ROWS);
@@ -426,7 +448,9 @@ static Wg8Plan wg8_plan(int64_t n_out, int kvol, int cin, int cout, int dtype) {
 
 extern "C" size_t d3d_act8_wgrad_workspace_bytes(int64_t n_out, int kvol, int cin, int cout, int dtype) {
   if (n_out < 1 || kvol < 1 || cin < 1 || cout < 1 || (dtype != D3D_F32 && dtype != D3D_BF16)) return 0;
-  const int splits = wg8_plan(n_out, kvol, cin, cout, dtype).splits;
+  // (with and without a table: the larger of the two)
+  const int s0 = wg8_plan(n_out, kvol, cin, cout, dtype, true).splits, s1 = wg8_plan(n_out, kvol, cin, cout, dtype, false).splits;
+  const int splits = s0 > s1 ? s0 : s1;
   return splits > 1 ? (size_t)splits * kvol * cin * cout * sizeof(float) : 0;
 }
 
@@ -445,12 +469,13 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   D3D_REQUIRE(dy_stride >= cout, "d3d_act8_wgrad: rows of %d channels %lld elements apart", cout, (long long)dy_stride);
   D3D_REQUIRE(nbr ? cap >= n_out : (kvol == 1 && n_in == n_out), "d3d_act8_wgrad: cap=%lld kvol=%d n_in=%lld n_out=%lld",
               (long long)cap, kvol, (long long)n_in, (long long)n_out);
-  D3D_REQUIRE(!nbr || n_in * a8_pitch(cin) < ((int64_t)1 << 31), "d3d_act8_wgrad: %lld held rows of %d channels behind a table take 2 GB or more",
-              (long long)n_in, cin);
+  D3D_REQUIRE(!nbr || (n_in * a8_pitch(cin) < ((int64_t)1 << 31) - 16 && n_in < (1 << 24) && kvol * cap < (1 << 29)),
+              "d3d_act8_wgrad: %lld held rows of %d channels behind a table of %d x %lld entries (below 2^24 rows, 2 GB of codes, 2 GB of table)",
+              (long long)n_in, cin, kvol, (long long)cap);
   const size_t need = d3d_act8_wgrad_workspace_bytes(n_out, kvol, cin, cout, dtype);
   if (need && (!workspace || workspace_bytes < need))
     return d3d_set_error(D3D_ECAPACITY, "d3d_act8_wgrad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  const Wg8Plan q = wg8_plan(n_out, kvol, cin, cout, dtype);
+  const Wg8Plan q = wg8_plan(n_out, kvol, cin, cout, dtype, nbr != nullptr);
   Wg8Args p;
   p.codes = codes;
   p.scales = scales;
@@ -461,6 +486,7 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   p.cap = cap;
   p.count = (int64_t)kvol * cin * cout;
   p.n_in = (uint32_t)n_in;
+  p.tab_bytes = nbr ? (uint32_t)(kvol * cap * 4) : 0u;
   p.n_out = (int)n_out;
   p.cin = cin;
   p.cinp = (cin + 7) / 8 * 8;
@@ -473,28 +499,29 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   p.chunks = q.chunks;
   p.per_split = q.per_split;
   const dim3 grid((unsigned)(q.groups * q.cotiles * q.splits));
-#define A8_WG(F, P, WCO, WK, NB)                                                                                                \
-  do {                                                                                                                          \
-    if (nbr && q.kg == 2) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 2, WG8_UB, true>), grid, dim3(512), 0, stream, p);  \
-    else if (nbr) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 4, WG8_UB, true>), grid, dim3(512), 0, stream, p);     \
-    else if (q.kg == 2) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 2, WG8_UB, false>), grid, dim3(512), 0, stream, p); \
-    else hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 4, WG8_UB, false>), grid, dim3(512), 0, stream, p);             \
+#define A8_WG(F, P, WCO, WK, NB, EDGE)                                                                                                    \
+  do {                                                                                                                                    \
+    if (nbr) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 4, WG8_UB, true, EDGE>), grid, dim3(512), 0, stream, p);              \
+    else if (q.kg == 2) hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 2, WG8_UB, false, EDGE>), grid, dim3(512), 0, stream, p);  \
+    else hipLaunchKernelGGL((a8_wgrad_kernel<F, P, WCO, WK, NB, 4, WG8_UB, false, EDGE>), grid, dim3(512), 0, stream, p);                 \
   } while (0)
-#define A8_WG_TN(F)                                                                                                             \
-  do {                                                                                                                          \
-    if (dtype == D3D_BF16) {                                                                                                    \
-      if (q.tn == 32) A8_WG(F, 1, 1, 4, 1);                                                                                     \
-      else if (q.tn == 64) A8_WG(F, 1, 2, 2, 1);                                                                                \
-      else if (q.tn == 128) A8_WG(F, 1, 4, 1, 1);                                                                               \
-      else A8_WG(F, 1, 4, 1, 2);                                                                                                \
-    } else {                                                                                                                    \
-      if (q.tn == 32) A8_WG(F, 3, 1, 4, 1);                                                                                     \
-      else if (q.tn == 64) A8_WG(F, 3, 2, 2, 1);                                                                                \
-      else A8_WG(F, 3, 4, 1, 1);                                                                                                \
-    }                                                                                                                           \
+#define A8_WG_TN(F, P, EDGE)                                                                                                              \
+  do {                                                                                                                                    \
+    if (q.tn == 32) A8_WG(F, P, 1, 4, 1, EDGE);                                                                                           \
+    else if (q.tn == 64) A8_WG(F, P, 2, 2, 1, EDGE);                                                                                      \
+    else if (q.tn == 128) A8_WG(F, P, 4, 1, 1, EDGE);                                                                                     \
+    else if constexpr (P == 1 && !EDGE) A8_WG(F, P, 4, 1, 2, EDGE);                                                                       \
   } while (0)
-  if (fmt == D3D_ACT8_INT8) A8_WG_TN(D3D_ACT8_INT8);
-  else A8_WG_TN(D3D_ACT8_E4M3);
+#define A8_WG_ALL(F)                                                                                                                      \
+  do {                                                                                                                                    \
+    if (dtype == D3D_BF16 && !q.edge) A8_WG_TN(F, 1, false);                                                                              \
+    else if (dtype == D3D_BF16) A8_WG_TN(F, 1, true);                                                                                     \
+    else if (!q.edge) A8_WG_TN(F, 3, false);                                                                                              \
+    else A8_WG_TN(F, 3, true);                                                                                                            \
+  } while (0)
+  if (fmt == D3D_ACT8_INT8) A8_WG_ALL(D3D_ACT8_INT8);
+  else A8_WG_ALL(D3D_ACT8_E4M3);
+#undef A8_WG_ALL
 #undef A8_WG_TN
 #undef A8_WG
   D3D_LAUNCH_TRY("a8_wgrad_kernel");

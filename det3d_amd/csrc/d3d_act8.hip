@@ -123,6 +123,20 @@ typedef __attribute__((ext_vector_type(8))) __bf16 a8_bf16x8;
 typedef __attribute__((ext_vector_type(16))) float a8_f32x16;
 
 #define WG8_ROWS 64
+#ifndef WG8_VPM
+#define WG8_VPM 6
+#endif
+#if WG8_VPM
+#define WG8_INTERLEAVE                                              \
+  if (ph == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2 * UB * KS + 2 * KS * NB * P, 0); \
+  else __builtin_amdgcn_sched_group_barrier(0x100, 2 * UB * KS, 0); \
+  _Pragma("unroll") for (int m = 0; m < UB * KS * NB * P; ++m) {    \
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);              \
+    __builtin_amdgcn_sched_group_barrier(0x002, WG8_VPM, 0);        \
+  }
+#else
+#define WG8_INTERLEAVE
+#endif
 
 struct Wg8Args {
   const uint8_t *codes, *scales;
@@ -188,7 +202,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   constexpr int VPT = TN >= 64 ? TN / 64 : 1;  // vectors of 8 columns of dy a thread stages
   constexpr int ABYTES = WG8_ROWS * 128, DBYTES = WG8_ROWS * TN * 2;
   constexpr int RBYTES = (WK - 1) * 2 * WCO * 4096;
-  constexpr int SMEM = 2 * UB * ABYTES + P * DBYTES > RBYTES ? 2 * UB * ABYTES + P * DBYTES : RBYTES;
+  constexpr int SMEM = 2 * UB * ABYTES + 2 * P * DBYTES > RBYTES ? 2 * UB * ABYTES + 2 * P * DBYTES : RBYTES;
   __shared__ __attribute__((aligned(16))) unsigned char smem[SMEM];
   unsigned char *const sa = smem, *const sd = smem + 2 * UB * ABYTES;
 
@@ -286,7 +300,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       if (dy_chunk * WG8_ROWS + r < rows_here) dyp[v] += (int64_t)WG8_ROWS * p.dy_stride * EB;
     }
   };
-  auto write_dy = [&]() {
+  auto write_dy = [&](int buf) {
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = tid + 512 * v, r = i / (TN / 8), cv = i % (TN / 8);
@@ -312,7 +326,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
         }
       }
 #pragma unroll
-      for (int q = 0; q < P; ++q) *(uint4 *)(sd + q * DBYTES + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+      for (int q = 0; q < P; ++q) *(uint4 *)(sd + (buf * P + q) * DBYTES + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
     }
   };
 
@@ -333,41 +347,58 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
     load_code(u, 0);
     load_idx(u, 1);
   }
-  for (int chunk = 0; chunk < chunks; ++chunk) {
-    auto stage = [&](int u) {
-      *(uint4 *)(sa + (u % (2 * UB)) * ABYTES + wg8_slot<64>(srow, sseg)) = wg8_restore<FMT>(code[u], sc[u]);
-      load_code(u, chunk + 1);  // (its index arrived a chunk ago)
-      load_idx(u, chunk + 2);
-    };
-    write_dy();
+  // the codes of unit u of chunk `of` into the half `h` of A; then its next loads (the index arrived a chunk ago)
+  auto stage = [&](int u, int of, int h) {
+    *(uint4 *)(sa + (h * UB + u % UB) * ABYTES + wg8_slot<64>(srow, sseg)) = wg8_restore<FMT>(code[u], sc[u]);
+    load_code(u, of + 1);
+    load_idx(u, of + 2);
+  };
+  constexpr int PH = KG / UB;
+  write_dy(0);
+  load_dy();
 #pragma unroll
-    for (int u = 0; u < UB; ++u) stage(u);
-    d3d_lds_barrier();
+  for (int u = 0; u < UB; ++u) stage(u, 0, 0);
+  d3d_lds_barrier();
+  // A phase multiplies UB units and meanwhile stages the next UB (behind the chunk's last: the next chunk's first, and its dy).
+  // Written with the vector work between the MFMAs, which leave its pipe free: done one after the other, MFMA, restoring and
+  // LDS add up (43 + 47 + 26 thousand cycles of 121 at 64 -> 64 channels, f32).
+  for (int chunk = 0; chunk < chunks; ++chunk) {
     a8_bf16x8 bf[KS][NB][P];
+    const unsigned char *const dcur = sd + (chunk & 1) * P * DBYTES;
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int q = 0; q < P; ++q) bf[k][n][q] = wg8_fragment<TN>(sd + q * DBYTES, (wk * KS + k) * 16, (wco * NB + n) * 32);
-    load_dy();
-    // (units behind the last are worked on too, with zeros: a branch around them would make every wait for a load a wait for all)
+        for (int q = 0; q < P; ++q) bf[k][n][q] = wg8_fragment<TN>(dcur + q * DBYTES, (wk * KS + k) * 16, (wco * NB + n) * 32);
 #pragma unroll
-    for (int u0 = 0; u0 < KG; u0 += UB) {
+    for (int ph = 0; ph < PH; ++ph) {
+      const int h = PH % 2 == 0 ? ph & 1 : chunk & 1;  // this phase's half of A
+      a8_bf16x8 af[UB][KS];
 #pragma unroll
-      for (int u = u0 + UB; u < u0 + 2 * UB && u < KG; ++u) stage(u);
+      for (int v = 0; v < UB; ++v)
 #pragma unroll
-      for (int u = u0; u < u0 + UB; ++u) {
-        a8_bf16x8 af[KS];
+        for (int k = 0; k < KS; ++k) af[v][k] = wg8_fragment<64>(sa + (h * UB + v) * ABYTES, (wk * KS + k) * 16, wci * 32);
+      // (units behind the last are worked on too, with zeros: a branch around them would make every wait for a load a wait for all)
+      if (ph + 1 < PH) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) af[k] = wg8_fragment<64>(sa + (u % (2 * UB)) * ABYTES, (wk * KS + k) * 16, wci * 32);
+        for (int v = 0; v < UB; ++v) stage((ph + 1) * UB + v, chunk, h ^ 1);
+      } else {
+        write_dy((chunk + 1) & 1);
+        load_dy();
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int q = P - 1; q >= 0; --q) acc[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[k], bf[k][n][q], acc[u][n], 0, 0, 0);
+        for (int v = 0; v < UB; ++v) stage(v, chunk + 1, h ^ 1);
       }
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int q = P - 1; q >= 0; --q)
+#pragma unroll
+          for (int v = 0; v < UB; ++v)
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+              acc[ph * UB + v][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[v][k], bf[k][n][q], acc[ph * UB + v][n], 0, 0, 0);
+      WG8_INTERLEAVE
       d3d_lds_barrier();
       __builtin_amdgcn_sched_barrier(0);
     }

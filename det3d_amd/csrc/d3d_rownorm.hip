@@ -44,7 +44,7 @@ struct RjArgs {
   D3dRowJoinGrads g;
   float inv_c;
   int pitch;
-  float *part;  // backward: [blocks][sums][c] when the grid has more than one block, else null
+  float *part;  // backward: the blocks' column sums, [blocks][rj_slabs(sums)][c]
   int sums;
 };
 
@@ -210,67 +210,89 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
   }
 }
 
-// the block's column sums: every lane's sums over the rows that it saw, added over the block's row groups in their order, into
-// the block's slab of the workspace (or, from a grid of one block, into the results)
+// The column sums of a launch: which pairs are asked for (bit 0: sum e fhat | sum e with e = act(g) dH, of which the gradients of
+// scale, post weight and post bias are multiples; bit 1: sum dz hhat | sum dz, those of pre weight and pre bias)
+__host__ __device__ static inline int rj_slabs(int sums) { return ((sums & 1) + (sums >> 1)) * 2; }
+
+// the block's: every lane's sums over the rows that it saw, added over the block's row groups in their order, into the block's slab
 template <int E, int T, int NV, int NT>
-__device__ __forceinline__ void rj_columns(const float *acc, int c, float *lds, float *dst) {
+__device__ __forceinline__ void rj_columns(const float *const *accs, int sums, int c, float *lds, float *dst) {
   constexpr int RPB = NT / T, EPL = E * NV;
   const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
-  if constexpr (RPB == 1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+  for (int a = 0; a < 4; ++a) {
+    if (!(sums >> (a / 2) & 1)) continue;
+    const float *acc = accs[a];
+    if constexpr (RPB == 1) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int at = (k * T + lane) * E + j;
-        if (at < c) dst[at] = acc[k * E + j];
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int at = (k * T + lane) * E + j;
+          if (at < c) dst[at] = acc[k * E + j];
+        }
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < E; ++j) lds[sub * (T * EPL) + (k * T + lane) * E + j] = acc[k * E + j];
+      __syncthreads();
+      for (int at = threadIdx.x; at < c; at += NT) {
+        float t = 0.f;
+#pragma unroll
+        for (int s = 0; s < RPB; ++s) t += lds[s * (T * EPL) + at];
+        dst[at] = t;
       }
-  } else {
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < E; ++j) lds[sub * (T * EPL) + (k * T + lane) * E + j] = acc[k * E + j];
-    __syncthreads();
-    for (int at = threadIdx.x; at < c; at += NT) {
-      float t = 0.f;
-#pragma unroll
-      for (int s = 0; s < RPB; ++s) t += lds[s * (T * EPL) + at];
-      dst[at] = t;
     }
+    dst += c;
   }
 }
 
+// E values of a [c] vector in LDS
+template <class S> __device__ __forceinline__ void rj_shared(const float *w, int at, float *v) {
+  if constexpr (S::E == 1) v[0] = w[at];
+  else {
+#pragma unroll
+    for (int j = 0; j < S::E; j += 4) *(float4 *)(v + j) = *(const float4 *)(w + at + j);
+  }
+}
+
+// The backward pass keeps x, f, act and dH of a row in registers, five column sums over the rows beside them (40 registers of a
+// lane with 8 values), and the [c] vectors in LDS: with those in registers too it takes 180 of them, two waves to a SIMD in
+// place of four, and [8192, 4096] bf16 took 201 us in place of 169.
 // HELD: 0 rows as they are, 1 + format: codes
-template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_bwd_kernel(RjArgs p) {
+template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4 && S::NT < 512 ? 3 : 4) row_join_bwd_kernel(RjArgs p) {
   constexpr int E = S::E, T = S::T, NV = S::NV, EB = S::BF16 ? 2 : 4;
   constexpr int FMT = HELD == 2 ? D3D_ACT8_E4M3 : D3D_ACT8_INT8;
   using Row = A8Row<S::BF16, E>;
   using Code = A8Held<FMT, E, 1>;
   using In = typename std::conditional<HELD != 0, Code, Row>::type;  // what x and f come as
   __shared__ float lds1[2][1][S::NT / 64], lds2[2][2][S::NT / 64], lds3[2][3][S::NT / 64];
-  __shared__ float cols[S::RPB > 1 ? S::NT * S::EPL : 1];
+  // post weight | post bias | alpha scale | pre weight; behind the rows the block's column sums
+  extern __shared__ __attribute__((aligned(16))) float vec[];
   int slot1 = 0, slot2 = 0, slot3 = 0;
   const D3dRowJoin &a = p.a;
   const D3dRowJoinGrads &g = p.g;
   const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
-  const int c = a.c;
+  const int c = a.c, cp = (c + 3) & ~3;
   const bool has_f = HELD ? a.f_codes != nullptr : a.f != nullptr;
-  float pw[S::EPL], pb[S::EPL], sc[S::EPL], qw[S::EPL];
-  if (has_f) {
-    rj_vector<S>(a.post_weight, 1.f, 1.f, lane, c, pw);
-    rj_vector<S>(a.post_bias, 0.f, 1.f, lane, c, pb);
-    rj_vector<S>(a.scale, 1.f, a.alpha, lane, c, sc);
+  float *const pw = vec, *const pb = vec + cp, *const sc = vec + 2 * cp, *const qw = vec + 3 * cp;
+  for (int i = threadIdx.x; i < c; i += S::NT) {
+    pw[i] = a.post_weight ? a.post_weight[i] : 1.f;
+    pb[i] = a.post_bias ? a.post_bias[i] : 0.f;
+    sc[i] = a.scale ? a.alpha * a.scale[i] : a.alpha;
+    qw[i] = a.pre_weight ? a.pre_weight[i] : 1.f;
   }
-  if (a.pre_kind) rj_vector<S>(a.pre_weight, 1.f, 1.f, lane, c, qw);
-  float s_scale[S::EPL], s_pw[S::EPL], s_pb[S::EPL], s_qw[S::EPL], s_qb[S::EPL];
+  __syncthreads();
+  float s_ef[S::EPL], s_e[S::EPL], s_qw[S::EPL], s_qb[S::EPL];
 #pragma unroll
-  for (int j = 0; j < S::EPL; ++j) s_scale[j] = s_pw[j] = s_pb[j] = s_qw[j] = s_qb[j] = 0.f;
+  for (int j = 0; j < S::EPL; ++j) s_ef[j] = s_e[j] = s_qw[j] = s_qb[j] = 0.f;
 
   for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
     const bool mine = base + sub < a.n;
     const int64_t row = mine ? base + sub : a.n - 1;
-    // every load of the row first.  A row behind the last takes part in the sums over lanes with zero gradients, so that it
-    // adds nothing to the columns
+    // every load of the row first.  A row behind the last takes part in the sums over lanes with zero gradients
     typename In::Raw rx[NV], rf[NV];
     typename Row::Raw rg[NV], rdh[NV], rdz[NV];
 #pragma unroll
@@ -291,7 +313,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
     float ag = 1.f, dag = 0.f;
     if (a.gate_cols == 1) A8Row<S::BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
 
-    float h[S::EPL], f[S::EPL], m[S::EPL], dm[S::EPL];  // x, then h, then hhat | f, then fhat | act(g) | act'(g)
+    float h[S::EPL], f[S::EPL];  // x, then h, then hhat | f, then fhat
 #pragma unroll
     for (int k = 0; k < NV; ++k) In::unpack(rx[k], h + k * E);
     float fr = 1.f;
@@ -309,25 +331,29 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
       }
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
+        const int at = (k * T + lane) * E;
+        float m[E], w[E], b[E], s[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          m[k * E + j] = ag;
-          dm[k * E + j] = 1.f;
+          m[j] = ag;
+          w[j] = b[j] = s[j] = 0.f;
         }
         if (a.gate_cols > 1) {
-          Row::unpack(rg[k], m + k * E);
+          float unused;
+          Row::unpack(rg[k], m);
           if (a.gate_act != D3D_GATE_NONE) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) rj_act<true>(a.gate_act, m[k * E + j], m[k * E + j], dm[k * E + j]);
+            for (int j = 0; j < E; ++j) rj_act<false>(a.gate_act, m[j], m[j], unused);
           }
         }
-        const bool in = (k * T + lane) * E < c;
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const int q = k * E + j;
-          const float v = fmaf(sc[q] * m[q], fmaf(f[q], pw[q], pb[q]), h[q]);
-          h[q] = in ? v : 0.f;
+        if (at < c) {
+          rj_shared<S>(pw, at, w);
+          rj_shared<S>(pb, at, b);
+          rj_shared<S>(sc, at, s);
         }
+#pragma unroll
+        for (int j = 0; j < E; ++j)  // (behind the row's end everything is zero)
+          h[k * E + j] = fmaf(s[j] * m[j], fmaf(f[k * E + j], w[j], b[j]), h[k * E + j]);
       }
     }
     float d[S::EPL];  // dH
@@ -336,13 +362,17 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
       float s2[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        float dz[E];
+        const int at = (k * T + lane) * E;
+        float dz[E], w[E];
         Row::unpack(rdz[k], dz);
+#pragma unroll
+        for (int j = 0; j < E; ++j) w[j] = 0.f;
+        if (at < c) rj_shared<S>(qw, at, w);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const int q = k * E + j;
           h[q] *= hr;
-          d[q] = dz[j] * qw[q];
+          d[q] = dz[j] * w[j];
           s2[0] = fmaf(d[q], h[q], s2[0]);
           s2[1] += d[q];
         }
@@ -378,20 +408,37 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
-      float dg[E];
+      float m[E], dm[E], dg[E], w[E], b[E], s[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        m[j] = ag;
+        dm[j] = 1.f;
+        w[j] = b[j] = s[j] = 0.f;
+      }
+      if (a.gate_cols > 1) {  // (act(g) and act'(g) from the gate as it came: cheaper than to keep them)
+        Row::unpack(rg[k], m);
+        if (a.gate_act != D3D_GATE_NONE) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) rj_act<true>(a.gate_act, m[j], m[j], dm[j]);
+        }
+      }
+      if (at < c) {
+        rj_shared<S>(pw, at, w);
+        rj_shared<S>(pb, at, b);
+        rj_shared<S>(sc, at, s);
+      }
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int q = k * E + j;
-        const float u = fmaf(f[q], pw[q], pb[q]), e = d[q] * m[q], du = e * sc[q];
-        dg[j] = d[q] * sc[q] * u;
+        const float e = d[q] * m[j];
+        dg[j] = d[q] * s[j] * fmaf(f[q], w[j], b[j]);
         s3[2] += dg[j];
-        dg[j] *= dm[q];
+        dg[j] *= dm[j];
         if (mine) {
-          s_scale[q] = fmaf(e, u, s_scale[q]);
-          s_pw[q] = fmaf(du, f[q], s_pw[q]);
-          s_pb[q] += du;
+          s_ef[q] = fmaf(e, f[q], s_ef[q]);
+          s_e[q] += e;
         }
-        d[q] = du * pw[q];
+        d[q] = e * s[j] * w[j];
         s3[0] = fmaf(d[q], f[q], s3[0]);
         s3[1] += d[q];
       }
@@ -413,49 +460,55 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT) row_join_b
       if (g.df && mine && at < c) Row::store(g.df, row * (int64_t)c + at, d + k * E);
     }
   }
-#pragma unroll
-  for (int j = 0; j < S::EPL; ++j) s_scale[j] *= a.alpha;
-  float *const results[5] = {g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
-  const float *const accs[5] = {s_scale, s_pw, s_pb, s_qw, s_qb};
-  int at = 0;
-#pragma unroll
-  for (int k = 0; k < 5; ++k) {
-    if (!results[k]) continue;
-    rj_columns<E, T, NV, S::NT>(accs[k], c, cols, p.part ? p.part + ((int64_t)blockIdx.x * p.sums + at) * c : results[k]);
-    ++at;
-  }
+  const float *const accs[4] = {s_ef, s_e, s_qw, s_qb};
+  if (p.sums) rj_columns<E, T, NV, S::NT>(accs, p.sums, c, vec, p.part + (int64_t)blockIdx.x * rj_slabs(p.sums) * c);
 }
 
-// the blocks' slabs added up: 32 columns a block, 32 parts of the slabs side by side, the parts in a tree.  (One thread a column
-// over all slabs took 117 us for 512 of them: as many dependent loads.)
-__global__ void __launch_bounds__(1024) row_join_fold_kernel(const float *__restrict__ part, int blocks, int sums, int c, D3dRowJoinGrads g) {
-  __shared__ float lds[32][33];
-  float *const all[5] = {g.dscale, g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int i = blockIdx.x * 32 + x;
-  const int64_t step = (int64_t)sums * c;
-  float t = 0.f;
-  if (i < sums * c) {
+// The blocks' slabs added up, 32 columns a block of threads, 32 parts of the slabs side by side, the parts in a tree (one thread a
+// column over all slabs took 117 us for 512 of them: as many dependent loads), and the gradients from the sums: with A = sum e fhat
+// and B = sum e,  ds = alpha (w A + b B),  dw = alpha s A,  db = alpha s B
+__global__ void __launch_bounds__(1024) row_join_fold_kernel(const float *__restrict__ part, int blocks, int sums, D3dRowJoin a, D3dRowJoinGrads g) {
+  __shared__ float lds[2][32][33];
+  const int c = a.c, slabs = rj_slabs(sums), x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int tiles = (c + 31) / 32, pair = blockIdx.x / tiles, i = blockIdx.x % tiles * 32 + x;
+  const int64_t step = (int64_t)slabs * c;
+  float t0 = 0.f, t1 = 0.f;
+  if (i < c) {
+    const float *src = part + (int64_t)pair * 2 * c + i;
 #pragma unroll 4
-    for (int b = y; b < blocks; b += 32) t += part[b * step + i];
+    for (int b = y; b < blocks; b += 32) {
+      t0 += src[b * step];
+      t1 += src[b * step + c];
+    }
   }
-  lds[y][x] = t;
+  lds[0][y][x] = t0;
+  lds[1][y][x] = t1;
   __syncthreads();
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) {
-    if (y < m) lds[y][x] += lds[y + m][x];
+    if (y < m) {
+      lds[0][y][x] += lds[0][y + m][x];
+      lds[1][y][x] += lds[1][y + m][x];
+    }
     __syncthreads();
   }
-  if (y != 0 || i >= sums * c) return;
-  int left = i / c;
-#pragma unroll
-  for (int k = 0; k < 5; ++k)
-    if (all[k] && left-- == 0) all[k][i % c] = lds[0][x];
+  if (y != 0 || i >= c) return;
+  t0 = lds[0][0][x];
+  t1 = lds[1][0][x];
+  if ((sums & 1) && pair == 0) {
+    const float s = a.scale ? a.alpha * a.scale[i] : a.alpha;
+    if (g.dscale) g.dscale[i] = a.alpha * fmaf(a.post_weight ? a.post_weight[i] : 1.f, t0, a.post_bias ? a.post_bias[i] * t1 : 0.f);
+    if (g.dpost_weight) g.dpost_weight[i] = s * t0;
+    if (g.dpost_bias) g.dpost_bias[i] = s * t1;
+  } else {
+    if (g.dpre_weight) g.dpre_weight[i] = t0;
+    if (g.dpre_bias) g.dpre_bias[i] = t1;
+  }
 }
 
 #define RJ_MAXC 8192
 static int rj_blocks_bwd(int64_t n, int rpb, int nt) {
-  const int64_t nb = (n + rpb - 1) / rpb, most = nt > 256 ? 512 : 1024;
+  const int64_t nb = (n + rpb - 1) / rpb, most = 256 * (1024 / nt);  // (four waves to a SIMD)
   return (int)(nb > most ? most : nb);
 }
 
@@ -554,7 +607,7 @@ extern "C" int d3d_row_join_fwd(const D3dRowJoin *a, d3d_stream_t stream_) {
 // workspace of the column sums: an upper bound over the row layouts (rows per block), which depend on alignment too
 extern "C" size_t d3d_row_join_ws_floats(int64_t n, int c, int dtype, int sums) {
   if (n < 1 || c < 1 || c > RJ_MAXC || sums < 1 || sums > 5 || (dtype != D3D_F32 && dtype != D3D_BF16)) return 0;
-  return (size_t)rj_blocks_bwd(n, 1, 256) * (size_t)sums * (size_t)c;
+  return (size_t)rj_blocks_bwd(n, 1, 256) * 4 * (size_t)c;
 }
 
 extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d3d_stream_t stream_) {
@@ -571,7 +624,7 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
   D3D_REQUIRE((!g->dscale || a->scale) && (!g->dpost_weight || a->post_weight) && (!g->dpost_bias || a->post_bias) &&
                   (!g->dpre_weight || a->pre_weight) && (!g->dpre_bias || a->pre_bias),
               "d3d_row_join_bwd: the gradient of an absent vector");
-  const int sums = !!g->dscale + !!g->dpost_weight + !!g->dpost_bias + !!g->dpre_weight + !!g->dpre_bias;
+  const int sums = (g->dscale || g->dpost_weight || g->dpost_bias ? 1 : 0) | (g->dpre_weight || g->dpre_bias ? 2 : 0);
   const bool vec = rj_vectors(a, g);
   RjArgs p;
   memset(&p, 0, sizeof(p));
@@ -585,23 +638,29 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
   rc = rj_for(a, vec, [&](auto shape) {
     using S = decltype(shape);
     blocks = rj_blocks_bwd(a->n, S::RPB, S::NT);
-    if (sums && blocks > 1) {
-      const size_t need = (size_t)blocks * sums * a->c;
+    if (sums) {
+      const size_t need = (size_t)blocks * rj_slabs(sums) * a->c;
       if (!g->ws || g->ws_floats < need)
         return d3d_set_error(D3D_ECAPACITY, "d3d_row_join_bwd: workspace of %zu floats, %zu needed", (size_t)g->ws_floats, need);
       p.part = g->ws;
     }
     const dim3 grid((unsigned)blocks), block(S::NT);
-    if (held == 0) hipLaunchKernelGGL((row_join_bwd_kernel<S, 0>), grid, block, 0, stream, p);
-    else if (held == 1) hipLaunchKernelGGL((row_join_bwd_kernel<S, 1>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((row_join_bwd_kernel<S, 2>), grid, block, 0, stream, p);
+    size_t lds = 4 * (size_t)((a->c + 3) & ~3);
+    if (S::RPB > 1 && lds < (size_t)S::NT * S::EPL) lds = (size_t)S::NT * S::EPL;
+    lds *= sizeof(float);
+    const void *fn = held == 0 ? (const void *)row_join_bwd_kernel<S, 0>
+                               : (held == 1 ? (const void *)row_join_bwd_kernel<S, 1> : (const void *)row_join_bwd_kernel<S, 2>);
+    if (lds > 48 * 1024) D3D_HIP_TRY(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (held == 0) hipLaunchKernelGGL((row_join_bwd_kernel<S, 0>), grid, block, lds, stream, p);
+    else if (held == 1) hipLaunchKernelGGL((row_join_bwd_kernel<S, 1>), grid, block, lds, stream, p);
+    else hipLaunchKernelGGL((row_join_bwd_kernel<S, 2>), grid, block, lds, stream, p);
     return D3D_OK;
   });
   if (rc) return rc;
   D3D_LAUNCH_TRY("row_join_bwd_kernel");
-  if (p.part) {
-    const int nb = (sums * a->c + 31) / 32;
-    hipLaunchKernelGGL(row_join_fold_kernel, dim3(nb), dim3(1024), 0, stream, p.part, blocks, sums, a->c, *g);
+  if (sums) {
+    const unsigned nb = (unsigned)((a->c + 31) / 32 * (rj_slabs(sums) / 2));
+    hipLaunchKernelGGL(row_join_fold_kernel, dim3(nb), dim3(1024), 0, stream, p.part, blocks, sums, *a, *g);
     D3D_LAUNCH_TRY("row_join_fold_kernel");
   }
   return D3D_OK;

@@ -45,98 +45,118 @@ def rows_of(t, what):
     other (any distance between rows; other layouts are copied)"""
     if not t.is_cuda:
         raise _lib.D3dError("%s runs on the GPU only (HIP kernels); got a %s tensor" % (what, t.device))
-    if t.dim() != 2:
-        raise _lib.D3dError("%s: rows [n, c] expected, got shape %s" % (what, tuple(t.shape)))
     if t.dtype not in _DT:
         raise _lib.D3dError("%s supports float32 / bfloat16 rows, got %s" % (what, t.dtype))
-    if t.shape[1] < 1:
+    if t.dim() != 2:
+        raise _lib.D3dError("%s: rows [n, c] expected, got shape %s" % (what, tuple(t.shape)))
+    n, c = t.shape
+    if c < 1:
         raise _lib.D3dError("%s: rows of no channels" % what)
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+    s0, s1 = t.stride()
+    if (s1 != 1 and c > 1) or (s0 < c and n > 1):
         t = t.contiguous()
     return t
 
 
 def row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    n, c = t.shape
+    return t.stride(0) if n > 1 else c
 
 
-class on_device:
-    """the device of the tensors as the current one for the launches of the block (a launch on a stream of another device
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def launch(what, dev, fn, *args):
+    """fn(*args, stream) on the current stream of `dev`, with `dev` as the current device (a launch on a stream of another device
     than the current one is an error of the runtime)"""
-
-    __slots__ = ("idx", "prev")
-
-    def __init__(self, dev):
-        self.idx = dev.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *exc):
-        if self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
-        return False
+    idx = dev.index
+    prev = _device()
+    if prev != idx:
+        torch.cuda.set_device(idx)
+    try:
+        rc = fn(*args, _lib.stream_ptr(idx))
+    finally:
+        if prev != idx:
+            torch.cuda.set_device(prev)
+    if rc:
+        _lib.check(rc, what)
 
 
 class Held:
-    """rows held in 8 bits: `codes` uint8 [n, pitch(c)], `scales` uint8 [n, pitch(c) / 32] (the biased exponent s + 127; 255: a
-    group that is restored as NaN), `shape`, the `dtype` they had, and `fmt`"""
+    """rows held in 8 bits: `shape`, the `dtype` they had, `fmt`, and one buffer with the `codes` (uint8 [n, pitch(c)]) and behind
+    them the `scales` (uint8 [n, pitch(c) / 32]: the biased exponent s + 127; 255: a group that is restored as NaN)"""
 
-    __slots__ = ("codes", "scales", "shape", "dtype", "fmt", "lease")
+    __slots__ = ("buf", "shape", "dtype", "fmt", "lease")
 
-    def __init__(self, codes, scales, shape, dtype, fmt, lease):
-        self.codes, self.scales, self.shape, self.dtype, self.fmt, self.lease = codes, scales, tuple(shape), dtype, fmt, lease
+    def __init__(self, buf, shape, dtype, fmt, lease):
+        self.buf, self.shape, self.dtype, self.fmt, self.lease = buf, shape, dtype, fmt, lease
+
+    @staticmethod
+    def room(n, c, dtype, fmt, dev, lease):
+        p = pitch(c)
+        return Held(mem.empty((n * (p + p // GROUP),), torch.uint8, dev, lease.arena), (n, c), dtype, fmt, lease)
+
+    @property
+    def codes(self):
+        n, c = self.shape
+        return self.buf[:n * pitch(c)].view(n, pitch(c))
+
+    @property
+    def scales(self):
+        n, c = self.shape
+        return self.buf[n * pitch(c):].view(n, pitch(c) // GROUP)
+
+    def pointers(self):
+        n, c = self.shape
+        p = self.buf.data_ptr()
+        return p, p + n * pitch(c)
 
     def meta(self):
-        """what Held(codes, scales, *meta) needs beside the two tensors (for autograd nodes, which keep tensors apart)"""
+        """what Held(buf, *meta) needs beside the buffer (for autograd nodes, which keep tensors apart)"""
         return self.shape, self.dtype, self.fmt, self.lease
 
     def check(self, what):
         return self.lease.check(what)
 
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self.buf.numel()
 
     def restore(self, dtype=None, out=None):
         """the rows again, in `dtype` (default: the one they had) or into `out` [n, c] (any distance between its rows)"""
         n, c = self.shape
         arena = self.check("act8.restore")
+        dev = self.buf.device
         if out is None:
-            out = mem.empty((n, c), self.dtype if dtype is None else dtype, self.codes.device, arena)
-        elif dtype is not None and dtype != out.dtype:
-            raise _lib.D3dError("act8.restore: dtype %s, but out is %s" % (dtype, out.dtype))
-        if out.dtype not in _DT:
-            raise _lib.D3dError("act8.restore writes float32 / bfloat16 rows, got %s" % out.dtype)
-        if tuple(out.shape) != (n, c) or out.device != self.codes.device or (c > 1 and out.stride(1) != 1) or \
-                (n > 1 and out.stride(0) < c):
-            raise _lib.D3dError("act8.restore: out must be [%d, %d] on %s with neighbouring channels next to each other and rows "
-                                "that do not overlap" % (n, c, self.codes.device))
-        if n == 0:
-            return out
-        dev = out.device
-        with on_device(dev):
-            _lib.check(_lib.lib().d3d_act8_restore(self.codes.data_ptr(), self.scales.data_ptr(), n, c, FORMATS[self.fmt],
-                                                   _DT[out.dtype], out.data_ptr(), row_stride(out), _lib.stream_ptr(dev)),
-                       "d3d_act8_restore")
+            dtype = self.dtype if dtype is None else dtype
+            if dtype not in _DT:
+                raise _lib.D3dError("act8.restore writes float32 / bfloat16 rows, got %s" % dtype)
+            out, stride = mem.empty((n, c), dtype, dev, arena), c
+        else:
+            if dtype is not None and dtype != out.dtype:
+                raise _lib.D3dError("act8.restore: dtype %s, but out is %s" % (dtype, out.dtype))
+            if out.dtype not in _DT:
+                raise _lib.D3dError("act8.restore writes float32 / bfloat16 rows, got %s" % out.dtype)
+            if tuple(out.shape) != (n, c) or out.device != dev or (c > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < c):
+                raise _lib.D3dError("act8.restore: out must be [%d, %d] on %s with neighbouring channels next to each other and "
+                                    "rows that do not overlap" % (n, c, dev))
+            stride = row_stride(out)
+        if n:
+            codes, scales = self.pointers()
+            launch("d3d_act8_restore", dev, _lib.lib().d3d_act8_restore, codes, scales, n, c, FORMATS[self.fmt], _DT[out.dtype],
+                   out.data_ptr(), stride)
         return out
 
 
 def hold(x, fmt="int8"):
     """`x` [n, c] in 8 bits.  Takes values only: nothing of the result carries a gradient."""
     f = format_id(fmt)
-    x = rows_of(x.detach(), "act8.hold")
+    x = rows_of(x, "act8.hold")
     n, c = x.shape
-    lease = mem.Lease()
-    dev, p = x.device, pitch(c)
-    codes = mem.empty((n, p), torch.uint8, dev, lease.arena)
-    scales = mem.empty((n, p // GROUP), torch.uint8, dev, lease.arena)
+    held = Held.room(n, c, x.dtype, fmt, x.device, mem.Lease())
     if n:
-        with on_device(dev):
-            _lib.check(_lib.lib().d3d_act8_hold(x.data_ptr(), row_stride(x), n, c, _DT[x.dtype], f, codes.data_ptr(),
-                                                scales.data_ptr(), _lib.stream_ptr(dev)), "d3d_act8_hold")
-    return Held(codes, scales, (n, c), x.dtype, fmt, lease)
+        codes, scales = held.pointers()
+        launch("d3d_act8_hold", x.device, _lib.lib().d3d_act8_hold, x.data_ptr(), row_stride(x), n, c, _DT[x.dtype], f, codes, scales)
+    return held
 
 
 def weight_grad(held, dy, nbr=None):
@@ -146,43 +166,42 @@ def weight_grad(held, dy, nbr=None):
         nbr None, n_out == n_in (a linear layer, a 1x1 convolution):  dw = x^T dy                     -> float32 [cin, cout]
 
     Entries of the table outside [0, n_in) are absent neighbours and add nothing.  Products are exact to float32 (bfloat16 `dy`: as
-    they are; float32 `dy`: in three bfloat16 terms), sums are float32 in a fixed order.  Non-finite values in `dy` make the
-    columns that they reach NaN."""
+    they are; float32 `dy`: in three bfloat16 terms), sums are float32 in a fixed order.  A non-finite value in `dy` makes NaN of its
+    column of dw, for every offset."""
     dy = rows_of(dy, "act8.weight_grad")
     n_in, cin = held.shape
     n_out, cout = dy.shape
     dev = dy.device
-    if held.codes.device != dev:
-        raise _lib.D3dError("act8.weight_grad: rows held on %s, dy on %s" % (held.codes.device, dev))
+    if held.buf.device != dev:
+        raise _lib.D3dError("act8.weight_grad: rows held on %s, dy on %s" % (held.buf.device, dev))
     if nbr is None:
         kvol, cap = 1, n_out
         if n_out != n_in:
             raise _lib.D3dError("act8.weight_grad: %d held rows, %d rows of dy and no table" % (n_in, n_out))
+        dw = torch.empty((cin, cout), dtype=torch.float32, device=dev)
     else:
         if nbr.dtype != torch.int32 or nbr.dim() != 2 or nbr.device != dev or not nbr.is_contiguous():
             raise _lib.D3dError("act8.weight_grad: nbr must be a contiguous int32 [kvol, cap] tensor on %s" % (dev,))
         kvol, cap = nbr.shape
         if kvol < 1 or cap < n_out:
             raise _lib.D3dError("act8.weight_grad: a table of %d x %d entries for %d rows of dy" % (kvol, cap, n_out))
-    dw = torch.empty((kvol, cin, cout), dtype=torch.float32, device=dev)
+        dw = torch.empty((kvol, cin, cout), dtype=torch.float32, device=dev)
     launch_weight_grad(held, dy, nbr.data_ptr() if nbr is not None else None, cap, kvol, dw)
-    return dw if nbr is not None else dw[0]
+    return dw
 
 
 def launch_weight_grad(held, dy, nbr_ptr, cap, kvol, dw):
-    """d3d_act8_wgrad on checked operands; `dw` contiguous float32 [kvol, cin, cout], overwritten"""
+    """d3d_act8_wgrad on checked operands; `dw` contiguous float32 of kvol * cin * cout values, overwritten"""
     L = _lib.lib()
     n_in, cin = held.shape
     n_out, cout = dy.shape
-    dev = dy.device
     arena = held.check("act8.weight_grad")
-    if n_out == 0 or n_in == 0:
+    if n_out == 0 or n_in == 0 or cout == 0:
         dw.zero_()
         return
-    dt = _DT[dy.dtype]
+    dev, dt = dy.device, _DT[dy.dtype]
     wsb = L.d3d_act8_wgrad_workspace_bytes(n_out, kvol, cin, cout, dt)
     ws = mem.empty((wsb,), torch.uint8, dev, arena) if wsb else None
-    with on_device(dev):
-        _lib.check(L.d3d_act8_wgrad(held.codes.data_ptr(), held.scales.data_ptr(), FORMATS[held.fmt], n_in, cin, dy.data_ptr(),
-                                    row_stride(dy), dt, n_out, cout, nbr_ptr, cap, kvol, dw.data_ptr(),
-                                    ws.data_ptr() if wsb else None, wsb, _lib.stream_ptr(dev)), "d3d_act8_wgrad")
+    codes, scales = held.pointers()
+    launch("d3d_act8_wgrad", dev, L.d3d_act8_wgrad, codes, scales, FORMATS[held.fmt], n_in, cin, dy.data_ptr(), row_stride(dy), dt,
+           n_out, cout, nbr_ptr, cap, kvol, dw.data_ptr(), ws.data_ptr() if wsb else None, wsb)

@@ -31,168 +31,179 @@ MAX_CHANNELS = 8192  # a row stays in registers
 
 NormSpec = collections.namedtuple("NormSpec", ("kind", "weight", "bias", "eps"))
 NormSpec.__doc__ = "a row norm: kind \"rms\" | \"layer\", float32 weight and bias [c] (either may be None), eps"
-_NONE = NormSpec(None, None, None, 0.0)
+_NONE = (0, 0.0, None, None)
 
 
 def _vector(t, c, dev, what):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != c or t.device != dev:
+    if t.dtype != torch.float32 or t.shape != (c,) or t.device != dev:
         raise _lib.D3dError("rownorm: %s must be float32 [%d] on %s, got %s %s on %s" % (what, c, dev, t.dtype, tuple(t.shape), t.device))
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _spec(norm, c, dev, what):
+    """(kind, eps, weight, bias) of a checked NormSpec / RowNorm / None"""
     if norm is None:
         return _NONE
-    if isinstance(norm, RowNorm):
-        norm = norm.spec
-    if norm.kind not in KINDS:
+    kind = KINDS.get(norm.kind)
+    if kind is None:
         raise ValueError("rownorm: kind %r of the %s norm, expected one of %s" % (norm.kind, what, sorted(KINDS)))
-    if not norm.eps >= 0:
+    eps = float(norm.eps)
+    if not eps >= 0:
         raise ValueError("rownorm: eps %r of the %s norm" % (norm.eps, what))
-    return NormSpec(norm.kind, _vector(norm.weight, c, dev, what + " weight"), _vector(norm.bias, c, dev, what + " bias"), float(norm.eps))
-
-
-class _Call:
-    """one call's operands, checked: what fills the D3dRowJoin of both directions"""
-
-    __slots__ = ("n", "c", "dtype", "dev", "post", "pre", "gate_cols", "act", "alpha", "fmt")
-
-    def __init__(self, x, f, post, pre, gate, gate_act, scale, alpha, checkpoint):
-        n, c = x.shape
-        if c > MAX_CHANNELS:
-            raise _lib.D3dError("rownorm: rows of %d channels, at most %d" % (c, MAX_CHANNELS))
-        self.n, self.c, self.dtype, self.dev = n, c, act8._DT[x.dtype], x.device
-        self.post, self.pre = _spec(post, c, x.device, "post"), _spec(pre, c, x.device, "pre")
-        if gate_act not in GATE_ACTS:
-            raise ValueError("rownorm.join: gate_act %r, expected one of %s" % (gate_act, sorted(GATE_ACTS)))
-        self.act, self.alpha = GATE_ACTS[gate_act], float(alpha)
-        self.fmt = None if checkpoint is None else checkpoint
-        if checkpoint is not None:
-            act8.format_id(checkpoint)
-        for t, what in ((f, "f"), (gate, "gate")):
-            if t is not None and (t.dtype != x.dtype or t.device != x.device):
-                raise _lib.D3dError("rownorm.join: %s is %s on %s, x %s on %s" % (what, t.dtype, t.device, x.dtype, x.device))
-        if f is not None and f.shape != x.shape:
-            raise _lib.D3dError("rownorm.join: x %s and f %s" % (tuple(x.shape), tuple(f.shape)))
-        self.gate_cols = 0
-        if gate is not None:
-            if gate.shape[0] != n or gate.shape[1] not in (1, c):
-                raise _lib.D3dError("rownorm.join: gate %s for rows %s: [n, c] or [n, 1]" % (tuple(gate.shape), (n, c)))
-            # (c == 1: one value a row either way)
-            self.gate_cols = gate.shape[1]
-
-    def desc(self, x, f, gate, scale, h, z, held=(None, None)):
-        hx, hf = held
-        p, q = self.post, self.pre
-        return _lib.RowJoin(
-            self.n, self.c, self.dtype, act8.FORMATS[self.fmt] if self.fmt else 0,
-            _dp(x), act8.row_stride(x) if x is not None else 0, _dp(f), act8.row_stride(f) if f is not None else 0,
-            _dp(gate), act8.row_stride(gate) if gate is not None else 0, self.gate_cols, self.act, _dp(scale), self.alpha,
-            KINDS.get(p.kind, 0), p.eps, _dp(p.weight), _dp(p.bias), KINDS.get(q.kind, 0), q.eps, _dp(q.weight), _dp(q.bias),
-            _dp(h), _dp(z),
-            hx.codes.data_ptr() if hx else None, hx.scales.data_ptr() if hx else None,
-            hf.codes.data_ptr() if hf else None, hf.scales.data_ptr() if hf else None)
+    return kind, eps, _vector(norm.weight, c, dev, what + " weight"), _vector(norm.bias, c, dev, what + " bias")
 
 
 def _dp(t):
     return None if t is None else t.data_ptr()
 
 
-def _forward(call, x, f, gate, scale, arena, held=(None, None)):
+def _rows(t):
+    """address and row stride of checked rows, (None, 0) of none"""
+    return (None, 0) if t is None else (t.data_ptr(), act8.row_stride(t))
+
+
+class _Call:
+    """what both directions of a call know beside the tensors"""
+
+    __slots__ = ("n", "c", "dtype", "dt", "dev", "post", "pre", "gate_cols", "act", "alpha", "fmt", "fmt_id", "has_f")
+
+    def desc(self, x, f, gate, scale, post, pre, h, z, hx, hf):
+        """the D3dRowJoin of a launch; post, pre: (weight, bias)"""
+        xc, xs = hx.pointers() if hx is not None else (None, None)
+        fc, fs = hf.pointers() if hf is not None else (None, None)
+        return _lib.RowJoin(self.n, self.c, self.dt, self.fmt_id, *_rows(x), *_rows(f), *_rows(gate), self.gate_cols, self.act,
+                            _dp(scale), self.alpha, self.post[0], self.post[1], _dp(post[0]), _dp(post[1]),
+                            self.pre[0], self.pre[1], _dp(pre[0]), _dp(pre[1]), _dp(h), _dp(z), xc, xs, fc, fs)
+
+
+def _call(x, f, post, pre, gate, gate_act, alpha, checkpoint):
+    call = _Call()
+    n, c = x.shape
+    dev, dtype = x.device, x.dtype
+    if c > MAX_CHANNELS:
+        raise _lib.D3dError("rownorm: rows of %d channels, at most %d" % (c, MAX_CHANNELS))
+    call.n, call.c, call.dtype, call.dt, call.dev, call.has_f = n, c, dtype, act8._DT[dtype], dev, f is not None
+    call.post, call.pre = _spec(post, c, dev, "post"), _spec(pre, c, dev, "pre")
+    call.act = GATE_ACTS.get(gate_act)
+    if call.act is None:
+        raise ValueError("rownorm.join: gate_act %r, expected one of %s" % (gate_act, sorted(GATE_ACTS)))
+    call.alpha = float(alpha)
+    call.fmt = checkpoint
+    call.fmt_id = 0 if checkpoint is None else act8.format_id(checkpoint)
+    call.gate_cols = 0
+    if f is not None and (f.dtype != dtype or f.device != dev or f.shape != x.shape):
+        raise _lib.D3dError("rownorm.join: x %s %s on %s and f %s %s on %s" % (dtype, tuple(x.shape), dev, f.dtype, tuple(f.shape), f.device))
+    if gate is not None:
+        call.gate_cols = gate.shape[1]
+        if gate.dtype != dtype or gate.device != dev or gate.shape[0] != n or (gate.shape[1] != c and gate.shape[1] != 1):
+            raise _lib.D3dError("rownorm.join: gate %s %s on %s for rows %s %s on %s: [n, c] or [n, 1] of x's type"
+                                % (gate.dtype, tuple(gate.shape), gate.device, dtype, (n, c), dev))
+    return call
+
+
+def _forward(call, x, f, gate, scale, post, pre, arena, hx=None, hf=None):
     n, c, dev = call.n, call.c, call.dev
-    h = mem.empty((n, c), x.dtype, dev, arena) if f is not None else None
-    z = mem.empty((n, c), x.dtype, dev, arena) if call.pre.kind else None
+    h = mem.empty((n, c), call.dtype, dev, arena) if f is not None else None
+    z = mem.empty((n, c), call.dtype, dev, arena) if call.pre[0] else None
     if n:
-        d = call.desc(x, f, gate, scale, h, z, held)
-        with act8.on_device(dev):
-            _lib.check(_lib.lib().d3d_row_join_fwd(ctypes.byref(d), _lib.stream_ptr(dev)), "d3d_row_join_fwd")
-    return h, z
+        d = call.desc(x, f, gate, scale, post, pre, h, z, hx, hf)
+        act8.launch("d3d_row_join_fwd", dev, _lib.lib().d3d_row_join_fwd, ctypes.byref(d))
+    if f is None:
+        return z
+    return h if z is None else (h, z)
 
 
 class _JoinFn(torch.autograd.Function):
     """both operators (f None: the norm alone); the weights travel as tensors of their own so that autograd sees them"""
 
     @staticmethod
-    def forward(ctx, x, f, gate, scale, post_w, post_b, pre_w, pre_b, call):
+    def forward(ctx, call, x, f, gate, scale, post_w, post_b, pre_w, pre_b):
         lease = mem.Lease()
         hx = hf = None
-        if call.fmt:
-            n, c, p = call.n, call.c, act8.pitch(call.c)
-
-            def room():
-                return act8.Held(mem.empty((n, p), torch.uint8, call.dev, lease.arena),
-                                 mem.empty((n, p // act8.GROUP), torch.uint8, call.dev, lease.arena), (n, c), x.dtype, call.fmt, lease)
-            hx, hf = room(), room() if f is not None else None
-        h, z = _forward(call, x, f, gate, scale, lease.arena, (hx, hf))
+        if call.fmt is not None:
+            hx = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease)
+            hf = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease) if f is not None else None
+        out = _forward(call, x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), lease.arena, hx, hf)
         ctx.set_materialize_grads(False)
-        ctx.call, ctx.lease, ctx.row_dtype, ctx.has_f = call, lease, x.dtype, f is not None
+        ctx.call, ctx.lease = call, lease
         # (in 8 bits the backward pass reads the codes alone: x and f are free once nobody else holds them)
-        held = () if hx is None else (hx.codes, hx.scales) + ((hf.codes, hf.scales) if hf is not None else ())
-        ctx.save_for_backward(*(held or (x, f)), gate, scale, post_w, post_b, pre_w, pre_b)
-        if f is None:
-            return z
-        return h if z is None else (h, z)
+        if hx is not None:
+            x, f = hx.buf, hf.buf if hf is not None else None
+        ctx.save_for_backward(x, f, gate, scale, post_w, post_b, pre_w, pre_b)
+        return out
 
     @staticmethod
     def backward(ctx, *grads):
         if torch.is_grad_enabled():
             raise _lib.D3dError("rownorm: its gradients have no derivatives of their own (create_graph)")
-        call, has_f = ctx.call, ctx.has_f
-        n, c, dev, dtype = call.n, call.c, call.dev, ctx.row_dtype
-        saved = ctx.saved_tensors
-        gate, scale, post_w, post_b, pre_w, pre_b = saved[-6:]
-        x = f = hx = hf = None
-        if call.fmt:
-            hx = act8.Held(saved[0], saved[1], (n, c), dtype, call.fmt, ctx.lease)
-            hf = act8.Held(saved[2], saved[3], (n, c), dtype, call.fmt, ctx.lease) if has_f else None
-        else:
-            x, f = saved[:2]
-        dh, dz = (grads[0] if has_f else None), (grads[-1] if call.pre.kind else None)
+        call = ctx.call
+        n, c, dev, dtype = call.n, call.c, call.dev, call.dtype
         arena = ctx.lease.check("rownorm")
-        need = ctx.needs_input_grad
+        x, f, gate, scale, post_w, post_b, pre_w, pre_b = ctx.saved_tensors
+        dh = dz = None
+        if call.has_f:
+            dh = grads[0]
+            if call.pre[0]:
+                dz = grads[1]
+        else:
+            dz = grads[0]
         if dh is None and dz is None:
             return (None,) * 9
-        dh, dz = (None if g is None else act8.rows_of(g if g.dtype == dtype else g.to(dtype), "rownorm") for g in (dh, dz))
-
-        def rows(wanted, cols=c):
-            return mem.empty((n, cols), dtype, dev, arena) if wanted else None
-
-        dx, df, dgate = rows(need[0]), rows(has_f and need[1]), rows(gate is not None and need[2], call.gate_cols)
+        if dh is not None:
+            dh = act8.rows_of(dh if dh.dtype == dtype else dh.to(dtype), "rownorm")
+        if dz is not None:
+            dz = act8.rows_of(dz if dz.dtype == dtype else dz.to(dtype), "rownorm")
+        hx = hf = None
+        if call.fmt is not None:
+            hx = act8.Held(x, (n, c), dtype, call.fmt, ctx.lease)
+            hf = act8.Held(f, (n, c), dtype, call.fmt, ctx.lease) if f is not None else None
+            x = f = None
+        _, need_x, need_f, need_g, need_s, need_pw, need_pb, need_qw, need_qb = ctx.needs_input_grad
+        dx = mem.empty((n, c), dtype, dev, arena) if need_x else None
+        df = mem.empty((n, c), dtype, dev, arena) if need_f else None
+        dgate = mem.empty((n, call.gate_cols), dtype, dev, arena) if need_g else None
         # scale, post weight, post bias, pre weight, pre bias: those that are asked for, each a row of one buffer
-        there = (scale, post_w, post_b, pre_w, pre_b)
-        want = [t is not None and need[3 + i] for i, t in enumerate(there)]
-        sums = list(torch.empty((sum(want), c), dtype=torch.float32, device=dev).unbind(0)) if any(want) else []
+        count = need_s + need_pw + need_pb + need_qw + need_qb
+        ds = dpw = dpb = dqw = dqb = None
+        if count:
+            sums = torch.empty((count, c), dtype=torch.float32, device=dev)
+            rows = sums.unbind(0)
+            at = 0
+            if need_s:
+                ds, at = rows[0], 1
+            if need_pw:
+                dpw, at = rows[at], at + 1
+            if need_pb:
+                dpb, at = rows[at], at + 1
+            if need_qw:
+                dqw, at = rows[at], at + 1
+            if need_qb:
+                dqb = rows[at]
         if n:
             L = _lib.lib()
-            ws = None
-            floats = 0
-            if sums:
-                floats = L.d3d_row_join_ws_floats(n, c, call.dtype, len(sums))
-                ws = mem.empty((floats,), torch.float32, dev, arena) if floats else None
-            d = call.desc(x, f, gate, scale, None, None, (hx, hf))
-            it = iter(sums)
-            ptrs = [next(it).data_ptr() if w else None for w in want]
-            g = _lib.RowJoinGrads(_dp(dh), act8.row_stride(dh) if dh is not None else 0, _dp(dz),
-                                  act8.row_stride(dz) if dz is not None else 0, _dp(dx), _dp(df), _dp(dgate), *ptrs, _dp(ws), floats)
-            with act8.on_device(dev):
-                _lib.check(L.d3d_row_join_bwd(ctypes.byref(d), ctypes.byref(g), _lib.stream_ptr(dev)), "d3d_row_join_bwd")
-        else:
-            for t in sums:
-                t.zero_()
-        it = iter(sums)
-        return (dx, df, dgate) + tuple(next(it) if w else None for w in want) + (None,)
+            ws, floats = None, 0
+            if count:
+                floats = L.d3d_row_join_ws_floats(n, c, call.dt, count)
+                ws = mem.empty((floats,), torch.float32, dev, arena)
+            d = call.desc(x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), None, None, hx, hf)
+            g = _lib.RowJoinGrads(*_rows(dh), *_rows(dz), _dp(dx), _dp(df), _dp(dgate), _dp(ds), _dp(dpw), _dp(dpb), _dp(dqw), _dp(dqb),
+                                  _dp(ws), floats)
+            act8.launch("d3d_row_join_bwd", dev, L.d3d_row_join_bwd, ctypes.byref(d), ctypes.byref(g))
+        elif count:
+            sums.zero_()
+        return None, dx, df, dgate, ds, dpw, dpb, dqw, dqb
 
 
-def _apply(x, f, gate, scale, call):
-    p, q = call.post, call.pre
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, f, gate, scale, p.weight, p.bias, q.weight, q.bias)):
-        return _JoinFn.apply(x, f, gate, scale, p.weight, p.bias, q.weight, q.bias, call)
-    h, z = _forward(call, x, f, gate, scale, None)
-    if f is None:
-        return z
-    return h if z is None else (h, z)
+def _apply(call, x, f, gate, scale):
+    _, _, pw, pb = call.post
+    _, _, qw, qb = call.pre
+    if torch.is_grad_enabled():
+        for t in (x, f, gate, scale, pw, pb, qw, qb):
+            if t is not None and t.requires_grad:
+                return _JoinFn.apply(call, x, f, gate, scale, pw, pb, qw, qb)
+    return _forward(call, x, f, gate, scale, (pw, pb), (qw, qb), None)
 
 
 def norm(x, spec, checkpoint=None):
@@ -200,7 +211,7 @@ def norm(x, spec, checkpoint=None):
     if spec is None:
         raise ValueError("rownorm.norm: no norm given")
     x = act8.rows_of(x, "rownorm.norm")
-    return _apply(x, None, None, None, _Call(x, None, None, spec, None, "none", None, 1.0, checkpoint))
+    return _apply(_call(x, None, None, spec, None, "none", 1.0, checkpoint), x, None, None, None)
 
 
 def join(x, f, post=None, pre=None, gate=None, gate_act="none", scale=None, alpha=1.0, checkpoint=None):
@@ -214,8 +225,8 @@ def join(x, f, post=None, pre=None, gate=None, gate_act="none", scale=None, alph
         gate = act8.rows_of(gate, "rownorm.join")
     elif gate_act != "none":
         raise ValueError("rownorm.join: gate_act %r without a gate" % (gate_act,))
-    call = _Call(x, f, post, pre, gate, gate_act, scale, alpha, checkpoint)
-    return _apply(x, f, gate, _vector(scale, x.shape[1], x.device, "scale"), call)
+    call = _call(x, f, post, pre, gate, gate_act, alpha, checkpoint)
+    return _apply(call, x, f, gate, _vector(scale, call.c, call.dev, "scale"))
 
 
 class RowNorm(nn.Module):

@@ -490,10 +490,10 @@ class _SparseConvFn(torch.autograd.Function):
         ctx.feat_dtype, ctx.held = feats.dtype, None
         if fmt is not None and ctx.needs_input_grad[1]:  # the weight gradient alone reads the input rows: keep them in 8 bits
             held = act8.hold(feats, fmt)
-            ctx.save_for_backward(held.codes, held.scales, weight)
+            ctx.save_for_backward(held.buf, weight)
             ctx.held = held.meta()
         else:
-            ctx.save_for_backward(feats, None, weight)
+            ctx.save_for_backward(feats, weight)
         ctx.wd = wd
         from . import repack
         ctx.repack_stamp = repack.stamp((weight,))  # `wd` is rewritten in place by Repacker.run()
@@ -509,7 +509,7 @@ class _SparseConvFn(torch.autograd.Function):
     @_lib.ctx_backward
     def backward(ctx, gout):
         L = _lib.lib()
-        feats, scales, weight = ctx.saved_tensors  # (held in 8 bits: codes, scales, weight)
+        feats, weight = ctx.saved_tensors  # (held in 8 bits: the buffer in place of feats)
         rb = ctx.rb
         kvol, cout = rb.kvol, weight.shape[-1]
         cin, pad_cin = ctx.pad
@@ -543,7 +543,7 @@ class _SparseConvFn(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             gw = torch.empty((kvol, pad_cin, cout), dtype=torch.float32, device=dev)
             if ctx.held is not None:
-                held = act8.Held(feats, scales, *ctx.held)
+                held = act8.Held(feats, *ctx.held)
                 _timed("wgrad", pad_cin, cout, rb.n_out, rb, dev, lambda: act8.launch_weight_grad(
                     held, gout, rb.nbr_out.data_ptr(), rb.cap_out, kvol, gw))
             else:
@@ -590,10 +590,10 @@ class _BNReLUFn(torch.autograd.Function):
         fmt, ctx.held = _runtime.held_format(), None
         if fmt is not None and training and link is None and any(ctx.needs_input_grad[:3]):
             held = act8.hold(x, fmt)
-            ctx.save_for_backward(held.codes, held.scales, weight, bias, save)
+            ctx.save_for_backward(held.buf, weight, bias, save)
             ctx.held = held.meta()
         else:
-            ctx.save_for_backward(x, None, weight, bias, save)
+            ctx.save_for_backward(x, weight, bias, save)
         ctx.relu = relu
         ctx.training = training
         ctx.link = link
@@ -611,9 +611,9 @@ class _BNReLUFn(torch.autograd.Function):
         if not ctx.training:
             raise _lib.D3dError("fused sparse BN backward is implemented for training mode only")
         L = _lib.lib()
-        x, scales, weight, bias, save = ctx.saved_tensors
+        x, weight, bias, save = ctx.saved_tensors
         if ctx.held is not None:
-            x = act8.Held(x, scales, *ctx.held).restore()
+            x = act8.Held(x, *ctx.held).restore()
         n, c = x.shape
         dy = dy.contiguous().to(x.dtype)
         A = ctx.lease.check("sparse BatchNorm")

@@ -73,9 +73,8 @@ __device__ __forceinline__ uint32_t a8_pack_bf16(float a, float b) {  // round t
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, a8_bf16x2));
 }
 
-// E neighbouring values of a row in the feature type: one 16-byte access (E = 4 f32 / 8 bf16), or one value (E = 1) where the
-// row is not aligned to 16 bytes or its width is no multiple of E.  Raw is what a load leaves in registers: loads issued early
-// and unpacked late stay in flight in between.
+// E neighbouring values of a row in the feature type: one 16-byte access (E = 4 f32 / 8 bf16), or one value (E = 1).  Raw is
+// what a load leaves in registers: loads issued early and unpacked late stay in flight in between.
 template <bool BF16, int E> struct A8Row {
   static_assert(E == 1 || E == (BF16 ? 8 : 4), "one value or one 16-byte vector");
   struct Raw {
@@ -111,6 +110,66 @@ template <bool BF16, int E> struct A8Row {
     }
   }
   __device__ static __forceinline__ void load(const void *row, int64_t at, float *v) { unpack(fetch(row, at), v); }
+  // The same on rows of any alignment and any width c, for vectors that begin inside the row: one that passes its end is read as
+  // the row's last E values and shifted into place (zeros behind the end), and written value by value.  hold of [100000, 127]:
+  // f32 26 us, bf16 20 us (one value a lane and load: 55 and 55; rows of 128: 24 and 17)
+  __device__ static __forceinline__ Raw fetch_any(const void *row, int at, int c) {
+    constexpr int EB = BF16 ? 2 : 4;
+    Raw r = zero();
+    if (c >= E) {
+      const uint4 q = a8_get<uint4>((const char *)row + (at + E <= c ? at : c - E) * EB);
+      r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+    } else {  // (a row shorter than a vector)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        if (at + j >= c) continue;
+        if constexpr (BF16) r.w[j / 2] |= (uint32_t)((const uint16_t *)row)[at + j] << (j % 2 * 16);
+        else r.w[j] = ((const uint32_t *)row)[at + j];
+      }
+    }
+    return r;
+  }
+  __device__ static __forceinline__ void unpack_any(const Raw &r, int at, int c, float *v) {
+    unpack(r, v);
+    const int s = at + E - c;
+    if (s > 0 && c >= E) {
+#pragma unroll
+      for (int m = 1; m < E; m <<= 1)
+        if (s & m) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[j] = j + m < E ? v[j + m] : 0.f;
+        }
+    }
+  }
+  __device__ static __forceinline__ void store_any(void *row, int at, int c, const float *v) {
+    constexpr int EB = BF16 ? 2 : 4;
+    if (at + E <= c) {
+      uint4 q;
+      if constexpr (BF16) q = make_uint4(a8_pack_bf16(v[0], v[1]), a8_pack_bf16(v[2], v[3]), a8_pack_bf16(v[4], v[5]), a8_pack_bf16(v[6], v[7]));
+      else q = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      a8_put((char *)row + at * EB, q);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (at + j < c) {
+          if constexpr (BF16) ((uint16_t *)row)[at + j] = (uint16_t)(a8_pack_bf16(v[j], 0.f) & 0xffffu);
+          else ((float *)row)[at + j] = v[j];
+        }
+    }
+  }
+  // one of the two: ANY = rows of any alignment and width
+  template <bool ANY> __device__ static __forceinline__ Raw get(const void *row, int at, int c) {
+    if constexpr (ANY) return fetch_any(row, at, c);
+    else return fetch(row, at);
+  }
+  template <bool ANY> __device__ static __forceinline__ void open(const Raw &r, int at, int c, float *v) {
+    if constexpr (ANY) unpack_any(r, at, c, v);
+    else unpack(r, v);
+  }
+  template <bool ANY> __device__ static __forceinline__ void put(void *row, int at, int c, const float *v) {
+    if constexpr (ANY) store_any(row, at, c, v);
+    else store(row, at, v);
+  }
   __device__ static __forceinline__ void store(void *row, int64_t at, const float *v) {
     if constexpr (E == 1) {
       if constexpr (BF16) ((uint16_t *)row)[at] = (uint16_t)(a8_pack_bf16(v[0], 0.f) & 0xffffu);
@@ -145,10 +204,7 @@ template <int FMT, int E, int LANES> struct A8Held {
     const float down = a8_down(b);
     if (!inside) return;
     uint8_t *c = codes + row * pitch + at;
-    if constexpr (E == 1) {
-      const float q[4] = {v[0], 0.f, 0.f, 0.f};
-      *c = (uint8_t)(a8_code4<FMT>(q, down) & 0xffu);
-    } else if constexpr (E == 4) {
+    if constexpr (E == 4) {
       *(uint32_t *)c = a8_code4<FMT>(v, down);
     } else {
       *(uint2 *)c = make_uint2(a8_code4<FMT>(v, down), a8_code4<FMT>(v + 4, down));
@@ -162,8 +218,7 @@ template <int FMT, int E, int LANES> struct A8Held {
     Raw r;
     r.b = scales[row * (pitch / A8_GROUP) + at / A8_GROUP];
     const uint8_t *c = codes + row * pitch + at;
-    if constexpr (E == 1) r.w[0] = *c;
-    else if constexpr (E == 4) r.w[0] = *(const uint32_t *)c;
+    if constexpr (E == 4) r.w[0] = *(const uint32_t *)c;
     else {
       const uint2 q = *(const uint2 *)c;
       r.w[0] = q.x;
@@ -180,14 +235,8 @@ template <int FMT, int E, int LANES> struct A8Held {
   }
   __device__ static __forceinline__ void unpack(const Raw &r, float *v) {
     const float up = a8_up(r.b);
-    if constexpr (E == 1) {
-      float q[4];
-      a8_value4<FMT>(r.w[0], up, q);
-      v[0] = q[0];
-    } else {
 #pragma unroll
-      for (int j = 0; j < E / 4; ++j) a8_value4<FMT>(r.w[j], up, v + 4 * j);
-    }
+    for (int j = 0; j < E / 4; ++j) a8_value4<FMT>(r.w[j], up, v + 4 * j);
   }
   __device__ static __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, int64_t row, int pitch, int at,
                                               float *v) {

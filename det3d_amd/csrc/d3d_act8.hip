@@ -1,13 +1,15 @@
 // Rows held in 8 bits, and the weight gradient that reads them (include/d3d.h, d3d_act8_*; arithmetic in d3d_act8.h).
 #include "d3d_act8.h"
 
-// ---- hold / restore: one pass over the rows, bound by HBM.  A lane moves one 16-byte vector (or one value of an unaligned row)
-// and the lanes of a group agree on its scale by shuffles.  Work items cover whole groups, so the codes behind the last channel
-// are written too (as zeros): what reads them later needs no mask.
-template <bool BF16, int E, int FMT>
+// ---- hold / restore: one pass over the rows, bound by HBM.  A lane moves one vector of 16 bytes and the lanes of a group agree
+// on its scale by shuffles.  Work items cover whole groups, so the codes behind the last channel are written too (as zeros):
+// what reads them later needs no mask.
+template <bool BF16, int FMT, bool ANY>
 __global__ void __launch_bounds__(256)
     a8_hold_kernel(const void *__restrict__ x, int64_t stride, int64_t n, int c, int pitch, uint8_t *__restrict__ codes,
                    uint8_t *__restrict__ scales) {
+  constexpr int E = BF16 ? 8 : 4, EB = BF16 ? 2 : 4;
+  using Row = A8Row<BF16, E>;
   const int per_row = pitch / E;
   const int64_t total = n * per_row;
   // (whole waves stay in the loop: every lane of a group takes part in its shuffles)
@@ -20,15 +22,16 @@ __global__ void __launch_bounds__(256)
     float v[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) v[j] = 0.f;
-    if (inside && at < c) A8Row<BF16, E>::load(x, row * stride + at, v);
+    if (inside && at < c) Row::template open<ANY>(Row::template get<ANY>((const char *)x + row * stride * EB, at, c), at, c, v);
     A8Held<FMT, E, A8_GROUP / E>::store(codes, scales, row, pitch, at, inside, v);
   }
 }
 
-template <bool BF16, int E, int FMT>
+template <bool BF16, int FMT, bool ANY>
 __global__ void __launch_bounds__(256)
     a8_restore_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t n, int c, int pitch,
                       void *__restrict__ out, int64_t stride) {
+  constexpr int E = BF16 ? 8 : 4, EB = BF16 ? 2 : 4;
   const int per_row = (c + E - 1) / E;
   const int64_t total = n * per_row;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -36,7 +39,7 @@ __global__ void __launch_bounds__(256)
     const int at = (int)(i - row * per_row) * E;
     float v[E];
     A8Held<FMT, E, A8_GROUP / E>::load(codes, scales, row, pitch, at, v);
-    A8Row<BF16, E>::store(out, row * stride + at, v);
+    A8Row<BF16, E>::template put<ANY>((char *)out + row * stride * EB, at, c, v);
   }
 }
 
@@ -51,23 +54,14 @@ static unsigned a8_grid(int64_t items) {
   return (unsigned)(nb < 1 ? 1 : (nb > 4096 ? 4096 : nb));
 }
 
-// KERNEL<type, vector width, format> by the row's type and alignment
-#define A8_LAUNCH(KERNEL, VEC, ITEMS_E, ...)                                                                             \
-  do {                                                                                                                   \
-    const dim3 grid(a8_grid(n * ((int64_t)(ITEMS_E) / ((VEC) ? (dtype == D3D_BF16 ? 8 : 4) : 1)))), block(256);          \
-    if (dtype == D3D_BF16 && (VEC)) {                                                                                    \
-      if (fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((KERNEL<true, 8, D3D_ACT8_INT8>), grid, block, 0, stream, __VA_ARGS__); \
-      else hipLaunchKernelGGL((KERNEL<true, 8, D3D_ACT8_E4M3>), grid, block, 0, stream, __VA_ARGS__);                    \
-    } else if (dtype == D3D_BF16) {                                                                                      \
-      if (fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((KERNEL<true, 1, D3D_ACT8_INT8>), grid, block, 0, stream, __VA_ARGS__); \
-      else hipLaunchKernelGGL((KERNEL<true, 1, D3D_ACT8_E4M3>), grid, block, 0, stream, __VA_ARGS__);                    \
-    } else if (VEC) {                                                                                                    \
-      if (fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((KERNEL<false, 4, D3D_ACT8_INT8>), grid, block, 0, stream, __VA_ARGS__); \
-      else hipLaunchKernelGGL((KERNEL<false, 4, D3D_ACT8_E4M3>), grid, block, 0, stream, __VA_ARGS__);                   \
-    } else {                                                                                                             \
-      if (fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((KERNEL<false, 1, D3D_ACT8_INT8>), grid, block, 0, stream, __VA_ARGS__); \
-      else hipLaunchKernelGGL((KERNEL<false, 1, D3D_ACT8_E4M3>), grid, block, 0, stream, __VA_ARGS__);                   \
-    }                                                                                                                    \
+// KERNEL<type, format, any alignment and width>
+#define A8_LAUNCH(KERNEL, ANY, ITEMS, ...)                                                                                          \
+  do {                                                                                                                              \
+    const dim3 grid(a8_grid(ITEMS)), block(256);                                                                                    \
+    if (dtype == D3D_BF16 && fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((KERNEL<true, D3D_ACT8_INT8, ANY>), grid, block, 0, stream, __VA_ARGS__); \
+    else if (dtype == D3D_BF16) hipLaunchKernelGGL((KERNEL<true, D3D_ACT8_E4M3, ANY>), grid, block, 0, stream, __VA_ARGS__);        \
+    else if (fmt == D3D_ACT8_INT8) hipLaunchKernelGGL((KERNEL<false, D3D_ACT8_INT8, ANY>), grid, block, 0, stream, __VA_ARGS__);    \
+    else hipLaunchKernelGGL((KERNEL<false, D3D_ACT8_E4M3, ANY>), grid, block, 0, stream, __VA_ARGS__);                              \
   } while (0)
 
 extern "C" int d3d_act8_pitch(int c) { return c >= 1 && c <= (1 << 20) ? a8_pitch(c) : 0; }
@@ -82,8 +76,9 @@ extern "C" int d3d_act8_hold(const void *x, int64_t x_stride, int64_t n, int c, 
   D3D_REQUIRE(x_stride >= c, "d3d_act8_hold: rows of %d channels %lld elements apart", c, (long long)x_stride);
   D3D_REQUIRE(((uintptr_t)codes & 15) == 0, "d3d_act8_hold: codes are not aligned to 16 bytes");
   const int pitch = a8_pitch(c);
-  const bool vec = a8_vectors(x, x_stride, c, dtype == D3D_BF16 ? 2 : 4);
-  A8_LAUNCH(a8_hold_kernel, vec, pitch, x, x_stride, n, c, pitch, codes, scales);
+  const int64_t items = n * (pitch / (dtype == D3D_BF16 ? 8 : 4));
+  if (a8_vectors(x, x_stride, c, dtype == D3D_BF16 ? 2 : 4)) A8_LAUNCH(a8_hold_kernel, false, items, x, x_stride, n, c, pitch, codes, scales);
+  else A8_LAUNCH(a8_hold_kernel, true, items, x, x_stride, n, c, pitch, codes, scales);
   D3D_LAUNCH_TRY("a8_hold_kernel");
   return D3D_OK;
 }
@@ -98,8 +93,10 @@ extern "C" int d3d_act8_restore(const uint8_t *codes, const uint8_t *scales, int
   D3D_REQUIRE(out_stride >= c, "d3d_act8_restore: rows of %d channels %lld elements apart", c, (long long)out_stride);
   D3D_REQUIRE(((uintptr_t)codes & 15) == 0, "d3d_act8_restore: codes are not aligned to 16 bytes");
   const int pitch = a8_pitch(c);
-  const bool vec = a8_vectors(out, out_stride, c, dtype == D3D_BF16 ? 2 : 4);
-  A8_LAUNCH(a8_restore_kernel, vec, vec ? c : c, codes, scales, n, c, pitch, out, out_stride);
+  const int e = dtype == D3D_BF16 ? 8 : 4;
+  const int64_t items = n * ((c + e - 1) / e);
+  if (a8_vectors(out, out_stride, c, dtype == D3D_BF16 ? 2 : 4)) A8_LAUNCH(a8_restore_kernel, false, items, codes, scales, n, c, pitch, out, out_stride);
+  else A8_LAUNCH(a8_restore_kernel, true, items, codes, scales, n, c, pitch, out, out_stride);
   D3D_LAUNCH_TRY("a8_restore_kernel");
   return D3D_OK;
 }

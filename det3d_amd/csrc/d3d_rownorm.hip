@@ -48,10 +48,10 @@ struct RjArgs {
   int sums;
 };
 
-// T lanes own a row, NV vectors of E values each; RPB rows to a block of NT threads
-template <bool BF16_, int E_, int T_, int NV_> struct RjShape {
-  static constexpr bool BF16 = BF16_;
-  static constexpr int E = E_, T = T_, NV = NV_;
+// T lanes own a row, NV vectors of E values each; RPB rows to a block of NT threads; ANY: rows of any alignment and width
+template <bool BF16_, int T_, int NV_, bool ANY_> struct RjShape {
+  static constexpr bool BF16 = BF16_, ANY = ANY_;
+  static constexpr int E = BF16_ ? 8 : 4, T = T_, NV = NV_;
   static constexpr int NT = T > 256 ? T : 256, RPB = NT / T, EPL = E * NV;
 };
 
@@ -67,24 +67,26 @@ template <bool DA> __device__ __forceinline__ void rj_act(int act, float g, floa
   }
 }
 
-// a [c] vector's values of this lane (`absent` where there is none), times `factor`; kept in registers over the rows
+// a [c] vector's values of this lane (`absent` where there is none, 0 behind its end), times `factor`; kept in registers over the rows
 template <class S> __device__ __forceinline__ void rj_vector(const float *w, float absent, float factor, int lane, int c, float *v) {
 #pragma unroll
   for (int k = 0; k < S::NV; ++k) {
     const int at = (k * S::T + lane) * S::E;
 #pragma unroll
-    for (int j = 0; j < S::E; ++j) v[k * S::E + j] = absent * factor;
-    if (w != nullptr && at < c) {
-      if constexpr (S::E == 1) v[k] = w[at] * factor;
-      else {
+    for (int j = 0; j < S::E; ++j) v[k * S::E + j] = at + j < c ? absent * factor : 0.f;
+    if (w == nullptr) continue;
+    if constexpr (S::ANY) {
 #pragma unroll
-        for (int j = 0; j < S::E; j += 4) {
-          const float4 q = *(const float4 *)(w + at + j);
-          v[k * S::E + j] = q.x * factor;
-          v[k * S::E + j + 1] = q.y * factor;
-          v[k * S::E + j + 2] = q.z * factor;
-          v[k * S::E + j + 3] = q.w * factor;
-        }
+      for (int j = 0; j < S::E; ++j)
+        if (at + j < c) v[k * S::E + j] = w[at + j] * factor;
+    } else if (at < c) {
+#pragma unroll
+      for (int j = 0; j < S::E; j += 4) {
+        const float4 q = *(const float4 *)(w + at + j);
+        v[k * S::E + j] = q.x * factor;
+        v[k * S::E + j + 1] = q.y * factor;
+        v[k * S::E + j + 2] = q.z * factor;
+        v[k * S::E + j + 3] = q.w * factor;
       }
     }
   }
@@ -102,9 +104,9 @@ __device__ __forceinline__ float rj_normalise(int kind, float eps, float inv_c, 
     const float mu = s[0] * inv_c;
 #pragma unroll
     for (int k = 0; k < S::NV; ++k) {
-      const float m = (k * S::T + lane) * S::E < c ? mu : 0.f;
+      const int at = (k * S::T + lane) * S::E;
 #pragma unroll
-      for (int j = 0; j < S::E; ++j) v[k * S::E + j] -= m;
+      for (int j = 0; j < S::E; ++j) v[k * S::E + j] -= (S::ANY ? at + j : at) < c ? mu : 0.f;
     }
   }
   float q[1] = {0.f};
@@ -115,7 +117,8 @@ __device__ __forceinline__ float rj_normalise(int kind, float eps, float inv_c, 
 }
 
 template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fwd_kernel(RjArgs p) {
-  constexpr int E = S::E, T = S::T, NV = S::NV;
+  constexpr int E = S::E, T = S::T, NV = S::NV, EB = S::BF16 ? 2 : 4;
+  constexpr bool ANY = S::ANY;
   constexpr int GL = A8_GROUP / E < T ? A8_GROUP / E : T;
   using Row = A8Row<S::BF16, E>;
   __shared__ float lds1[2][1][S::NT / 64];
@@ -143,14 +146,14 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
       const bool in = at < c;
-      rx[k] = in ? Row::fetch((const char *)a.x + row * a.x_stride * (S::BF16 ? 2 : 4), at) : Row::zero();
-      if (a.f) rf[k] = in ? Row::fetch((const char *)a.f + row * a.f_stride * (S::BF16 ? 2 : 4), at) : Row::zero();
-      if (a.gate_cols > 1) rg[k] = in ? Row::fetch((const char *)a.gate + row * a.gate_stride * (S::BF16 ? 2 : 4), at) : Row::zero();
+      rx[k] = in ? Row::template get<ANY>((const char *)a.x + row * a.x_stride * EB, at, c) : Row::zero();
+      if (a.f) rf[k] = in ? Row::template get<ANY>((const char *)a.f + row * a.f_stride * EB, at, c) : Row::zero();
+      if (a.gate_cols > 1) rg[k] = in ? Row::template get<ANY>((const char *)a.gate + row * a.gate_stride * EB, at, c) : Row::zero();
     }
     if (a.gate_cols == 1) A8Row<S::BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
     float h[S::EPL];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) Row::unpack(rx[k], h + k * E);
+    for (int k = 0; k < NV; ++k) Row::template open<ANY>(rx[k], (k * T + lane) * E, c, h + k * E);
     if (a.x_codes) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -161,7 +164,7 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
     if (a.f) {
       float f[S::EPL];
 #pragma unroll
-      for (int k = 0; k < NV; ++k) Row::unpack(rf[k], f + k * E);
+      for (int k = 0; k < NV; ++k) Row::template open<ANY>(rf[k], (k * T + lane) * E, c, f + k * E);
       if (a.f_codes) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -177,8 +180,9 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
         float g[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) g[j] = ag;
+        const int at = (k * T + lane) * E;
         if (a.gate_cols > 1) {
-          Row::unpack(rg[k], g);
+          Row::template open<ANY>(rg[k], at, c, g);
           if (a.gate_act != D3D_GATE_NONE) {
 #pragma unroll
             for (int j = 0; j < E; ++j) rj_act<false>(a.gate_act, g[j], g[j], dag);
@@ -189,12 +193,7 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
           const int q = k * E + j;
           h[q] = fmaf(sc[q] * g[j], fmaf(f[q] * r, pw[q], pb[q]), h[q]);
         }
-        const int at = (k * T + lane) * E;
-        if (mine && at < c) Row::store(a.h, row * (int64_t)c + at, h + k * E);
-        if (at >= c) {
-#pragma unroll
-          for (int j = 0; j < E; ++j) h[k * E + j] = 0.f;
-        }
+        if (mine && at < c) Row::template put<ANY>((char *)a.h + row * c * EB, at, c, h + k * E);
       }
     }
     if (a.pre_kind) {
@@ -204,7 +203,7 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
         const int at = (k * T + lane) * E;
 #pragma unroll
         for (int j = 0; j < E; ++j) h[k * E + j] = fmaf(h[k * E + j] * r, qw[k * E + j], qb[k * E + j]);
-        if (mine && at < c) Row::store(a.z, row * (int64_t)c + at, h + k * E);
+        if (mine && at < c) Row::template put<ANY>((char *)a.z + row * c * EB, at, c, h + k * E);
       }
     }
   }
@@ -249,13 +248,12 @@ __device__ __forceinline__ void rj_columns(const float *const *accs, int sums, i
   }
 }
 
+// the [c] vectors' length in LDS: whole vectors of either type
+__host__ __device__ static inline int rj_padded(int c) { return (c + 7) & ~7; }
 // E values of a [c] vector in LDS
 template <class S> __device__ __forceinline__ void rj_shared(const float *w, int at, float *v) {
-  if constexpr (S::E == 1) v[0] = w[at];
-  else {
 #pragma unroll
-    for (int j = 0; j < S::E; j += 4) *(float4 *)(v + j) = *(const float4 *)(w + at + j);
-  }
+  for (int j = 0; j < S::E; j += 4) *(float4 *)(v + j) = *(const float4 *)(w + at + j);
 }
 
 // The backward pass keeps x, f, act and dH of a row in registers, five column sums over the rows beside them (40 registers of a
@@ -264,6 +262,7 @@ template <class S> __device__ __forceinline__ void rj_shared(const float *w, int
 // HELD: 0 rows as they are, 1 + format: codes
 template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4 && S::NT < 512 ? 3 : 4) row_join_bwd_kernel(RjArgs p) {
   constexpr int E = S::E, T = S::T, NV = S::NV, EB = S::BF16 ? 2 : 4;
+  constexpr bool ANY = S::ANY;
   constexpr int FMT = HELD == 2 ? D3D_ACT8_E4M3 : D3D_ACT8_INT8;
   using Row = A8Row<S::BF16, E>;
   using Code = A8Held<FMT, E, 1>;
@@ -275,14 +274,15 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
   const D3dRowJoin &a = p.a;
   const D3dRowJoinGrads &g = p.g;
   const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
-  const int c = a.c, cp = (c + 3) & ~3;
+  const int c = a.c, cp = rj_padded(c);
   const bool has_f = HELD ? a.f_codes != nullptr : a.f != nullptr;
   float *const pw = vec, *const pb = vec + cp, *const sc = vec + 2 * cp, *const qw = vec + 3 * cp;
-  for (int i = threadIdx.x; i < c; i += S::NT) {
-    pw[i] = a.post_weight ? a.post_weight[i] : 1.f;
-    pb[i] = a.post_bias ? a.post_bias[i] : 0.f;
-    sc[i] = a.scale ? a.alpha * a.scale[i] : a.alpha;
-    qw[i] = a.pre_weight ? a.pre_weight[i] : 1.f;
+  for (int i = threadIdx.x; i < cp; i += S::NT) {
+    const bool in = i < c;
+    pw[i] = !in ? 0.f : (a.post_weight ? a.post_weight[i] : 1.f);
+    pb[i] = !in ? 0.f : (a.post_bias ? a.post_bias[i] : 0.f);
+    sc[i] = !in ? 0.f : (a.scale ? a.alpha * a.scale[i] : a.alpha);
+    qw[i] = !in ? 0.f : (a.pre_weight ? a.pre_weight[i] : 1.f);
   }
   __syncthreads();
   float s_ef[S::EPL], s_e[S::EPL], s_qw[S::EPL], s_qb[S::EPL];
@@ -303,23 +303,29 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
         rx[k] = in ? Code::fetch(a.x_codes, a.x_scales, row, p.pitch, at) : Code::zero();
         if (has_f) rf[k] = in ? Code::fetch(a.f_codes, a.f_scales, row, p.pitch, at) : Code::zero();
       } else {
-        rx[k] = in ? Row::fetch((const char *)a.x + row * a.x_stride * EB, at) : Row::zero();
-        if (has_f) rf[k] = in ? Row::fetch((const char *)a.f + row * a.f_stride * EB, at) : Row::zero();
+        rx[k] = in ? Row::template get<ANY>((const char *)a.x + row * a.x_stride * EB, at, c) : Row::zero();
+        if (has_f) rf[k] = in ? Row::template get<ANY>((const char *)a.f + row * a.f_stride * EB, at, c) : Row::zero();
       }
-      rg[k] = in && a.gate_cols > 1 ? Row::fetch((const char *)a.gate + row * a.gate_stride * EB, at) : Row::zero();
-      rdz[k] = in && mine && g.dz ? Row::fetch((const char *)g.dz + row * g.dz_stride * EB, at) : Row::zero();
-      rdh[k] = in && mine && g.dh ? Row::fetch((const char *)g.dh + row * g.dh_stride * EB, at) : Row::zero();
+      rg[k] = in && a.gate_cols > 1 ? Row::template get<ANY>((const char *)a.gate + row * a.gate_stride * EB, at, c) : Row::zero();
+      rdz[k] = in && mine && g.dz ? Row::template get<ANY>((const char *)g.dz + row * g.dz_stride * EB, at, c) : Row::zero();
+      rdh[k] = in && mine && g.dh ? Row::template get<ANY>((const char *)g.dh + row * g.dh_stride * EB, at, c) : Row::zero();
     }
     float ag = 1.f, dag = 0.f;
     if (a.gate_cols == 1) A8Row<S::BF16, 1>::load(a.gate, row * a.gate_stride, &ag);
 
     float h[S::EPL], f[S::EPL];  // x, then h, then hhat | f, then fhat
 #pragma unroll
-    for (int k = 0; k < NV; ++k) In::unpack(rx[k], h + k * E);
+    for (int k = 0; k < NV; ++k) {
+      if constexpr (HELD != 0) Code::unpack(rx[k], h + k * E);
+      else Row::template open<ANY>(rx[k], (k * T + lane) * E, c, h + k * E);
+    }
     float fr = 1.f;
     if (has_f) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) In::unpack(rf[k], f + k * E);
+      for (int k = 0; k < NV; ++k) {
+        if constexpr (HELD != 0) Code::unpack(rf[k], f + k * E);
+        else Row::template open<ANY>(rf[k], (k * T + lane) * E, c, f + k * E);
+      }
       if (a.post_kind) {
         fr = rj_normalise<S>(a.post_kind, a.post_eps, p.inv_c, lane, c, f, lds1, slot1);
 #pragma unroll
@@ -340,7 +346,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
         }
         if (a.gate_cols > 1) {
           float unused;
-          Row::unpack(rg[k], m);
+          Row::template open<ANY>(rg[k], at, c, m);
           if (a.gate_act != D3D_GATE_NONE) {
 #pragma unroll
             for (int j = 0; j < E; ++j) rj_act<false>(a.gate_act, m[j], m[j], unused);
@@ -364,7 +370,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
       for (int k = 0; k < NV; ++k) {
         const int at = (k * T + lane) * E;
         float dz[E], w[E];
-        Row::unpack(rdz[k], dz);
+        Row::template open<ANY>(rdz[k], at, c, dz);
 #pragma unroll
         for (int j = 0; j < E; ++j) w[j] = 0.f;
         if (at < c) rj_shared<S>(qw, at, w);
@@ -397,11 +403,11 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
       float dh[E];
-      Row::unpack(rdh[k], dh);
+      Row::template open<ANY>(rdh[k], at, c, dh);
       const bool in = at < c;
 #pragma unroll
       for (int j = 0; j < E; ++j) d[k * E + j] = in ? d[k * E + j] + dh[j] : 0.f;
-      if (g.dx && mine && in) Row::store(g.dx, row * (int64_t)c + at, d + k * E);
+      if (g.dx && mine && in) Row::template put<ANY>((char *)g.dx + row * c * EB, at, c, d + k * E);
     }
     if (!has_f) continue;
     float s3[3] = {0.f, 0.f, 0.f};
@@ -416,7 +422,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
         w[j] = b[j] = s[j] = 0.f;
       }
       if (a.gate_cols > 1) {  // (act(g) and act'(g) from the gate as it came: cheaper than to keep them)
-        Row::unpack(rg[k], m);
+        Row::template open<ANY>(rg[k], at, c, m);
         if (a.gate_act != D3D_GATE_NONE) {
 #pragma unroll
           for (int j = 0; j < E; ++j) rj_act<true>(a.gate_act, m[j], m[j], dm[j]);
@@ -442,7 +448,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
         s3[0] = fmaf(d[q], f[q], s3[0]);
         s3[1] += d[q];
       }
-      if (g.dgate && a.gate_cols > 1 && mine && at < c) Row::store(g.dgate, row * (int64_t)c + at, dg);
+      if (g.dgate && a.gate_cols > 1 && mine && at < c) Row::template put<ANY>((char *)g.dgate + row * c * EB, at, c, dg);
     }
     row_sum<T, S::NT, 3>(s3, lds3, slot3);
     if (g.dgate && a.gate_cols == 1 && mine && lane == 0) {
@@ -457,7 +463,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
 #pragma unroll
         for (int j = 0; j < E; ++j) d[k * E + j] = fr * (fmaf(-f[k * E + j], m2, d[k * E + j]) - m1);
       }
-      if (g.df && mine && at < c) Row::store(g.df, row * (int64_t)c + at, d + k * E);
+      if (g.df && mine && at < c) Row::template put<ANY>((char *)g.df + row * c * EB, at, c, d + k * E);
     }
   }
   const float *const accs[4] = {s_ef, s_e, s_qw, s_qb};
@@ -551,32 +557,24 @@ static bool rj_vectors(const D3dRowJoin *a, const D3dRowJoinGrads *g) {
   return v;
 }
 
-// The shape of the launch by the number of units (16-byte vectors, or values of unaligned rows) in a row: the fewest lanes that
-// hold it with at most 8 values a lane.  go(RjShape) launches.
-template <bool BF16, class Go> static int rj_pick(int c, bool vec, Go &&go) {
-  constexpr int E = BF16 ? 8 : 4;
-  if (vec) {
-    const int units = c / E;
-    if (units <= 8) return go(RjShape<BF16, E, 8, 1>{});
-    if (units <= 16) return go(RjShape<BF16, E, 16, 1>{});
-    if (units <= 32) return go(RjShape<BF16, E, 32, 1>{});
-    if (units <= 64) return go(RjShape<BF16, E, 64, 1>{});
-    if (units <= 128) return go(RjShape<BF16, E, 128, 1>{});
-    if (units <= 256) return go(RjShape<BF16, E, 256, 1>{});
-    if (units <= 512) return go(RjShape<BF16, E, 512, 1>{});
-    if (units <= 1024) return go(RjShape<BF16, E, BF16 ? 1024 : 512, BF16 ? 1 : 2>{});
-    return go(RjShape<BF16, E, 1024, BF16 ? 1 : 2>{});
-  }
-  if (c <= 32) return go(RjShape<BF16, 1, 32, 1>{});
-  if (c <= 64) return go(RjShape<BF16, 1, 64, 1>{});
-  if (c <= 128) return go(RjShape<BF16, 1, 64, 2>{});
-  if (c <= 256) return go(RjShape<BF16, 1, 64, 4>{});
-  if (c <= 512) return go(RjShape<BF16, 1, 64, 8>{});
-  if (c <= 2048) return go(RjShape<BF16, 1, 256, 8>{});
-  return go(RjShape<BF16, 1, 1024, 8>{});
+// The shape of the launch by the number of 16-byte vectors in a row: the fewest lanes that hold it with at most 8 values a lane.
+// go(RjShape) launches.
+template <bool BF16, bool ANY, class Go> static int rj_pick(int c, Go &&go) {
+  const int units = (c + (BF16 ? 8 : 4) - 1) / (BF16 ? 8 : 4);
+  if (units <= 8) return go(RjShape<BF16, 8, 1, ANY>{});
+  if (units <= 16) return go(RjShape<BF16, 16, 1, ANY>{});
+  if (units <= 32) return go(RjShape<BF16, 32, 1, ANY>{});
+  if (units <= 64) return go(RjShape<BF16, 64, 1, ANY>{});
+  if (units <= 128) return go(RjShape<BF16, 128, 1, ANY>{});
+  if (units <= 256) return go(RjShape<BF16, 256, 1, ANY>{});
+  if (units <= 512) return go(RjShape<BF16, 512, 1, ANY>{});
+  if constexpr (BF16) return go(RjShape<BF16, 1024, 1, ANY>{});
+  else if (units <= 1024) return go(RjShape<BF16, 512, 2, ANY>{});
+  else return go(RjShape<BF16, 1024, 2, ANY>{});
 }
 template <class Go> static int rj_for(const D3dRowJoin *a, bool vec, Go &&go) {
-  return a->dtype == D3D_BF16 ? rj_pick<true>(a->c, vec, go) : rj_pick<false>(a->c, vec, go);
+  if (a->dtype == D3D_BF16) return vec ? rj_pick<true, false>(a->c, go) : rj_pick<true, true>(a->c, go);
+  return vec ? rj_pick<false, false>(a->c, go) : rj_pick<false, true>(a->c, go);
 }
 
 extern "C" int d3d_row_join_fwd(const D3dRowJoin *a, d3d_stream_t stream_) {
@@ -645,7 +643,7 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
       p.part = g->ws;
     }
     const dim3 grid((unsigned)blocks), block(S::NT);
-    size_t lds = 4 * (size_t)((a->c + 3) & ~3);
+    size_t lds = 4 * (size_t)rj_padded(a->c);
     if (S::RPB > 1 && lds < (size_t)S::NT * S::EPL) lds = (size_t)S::NT * S::EPL;
     lds *= sizeof(float);
     const void *fn = held == 0 ? (const void *)row_join_bwd_kernel<S, 0>

@@ -166,8 +166,9 @@ def weight_grad(held, dy, nbr=None):
         nbr None, n_out == n_in (a linear layer, a 1x1 convolution):  dw = x^T dy                     -> float32 [cin, cout]
 
     Entries of the table outside [0, n_in) are absent neighbours and add nothing.  Products are exact to float32 (bfloat16 `dy`: as
-    they are; float32 `dy`: in three bfloat16 terms), sums are float32 in a fixed order.  A non-finite value in `dy` makes NaN of its
-    column of dw, for every offset."""
+    they are; float32 `dy`: in three bfloat16 terms), sums are float32 in a fixed order.  A non-finite value in `dy` (float32:
+    also one beyond bfloat16's range, 3.39e38) makes its column of dw non-finite, for every offset: rows meet an absent neighbour as
+    a zero."""
     dy = rows_of(dy, "act8.weight_grad")
     n_in, cin = held.shape
     n_out, cout = dy.shape

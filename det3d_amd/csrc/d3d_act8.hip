@@ -170,6 +170,9 @@ template <int FMT> __device__ __forceinline__ uint4 wg8_restore(uint2 w, uint32_
   }
 }
 
+// (a function: a conditional between two array elements would choose between their addresses, and put the array in memory)
+__device__ __forceinline__ uint32_t wg8_pick(int c, uint32_t a, uint32_t b) { return c ? a : b; }
+
 // byte of 16-byte slot `slot` in row r of a [rows][W columns] bf16 tile.  The slots of a row are permuted so that the four rows
 // of a transposing read (64 bytes each) lie in different banks: 128-byte rows alternate halves every second row, wider ones
 // rotate quarters of 256 bytes
@@ -193,7 +196,7 @@ template <int W> __device__ __forceinline__ a8_bf16x8 wg8_fragment(const unsigne
   return __builtin_bit_cast(a8_bf16x8, v);
 }
 
-template <int FMT, int P, int WCO, int WK, int NB, int KG, int UB, bool TABLE, bool EDGE>
+template <int FMT, int P, int WCO, int WK, int NB, int KG, int UB, bool TABLE, int EDGE>
 __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   constexpr int TN = WCO * NB * 32, KS = WG8_ROWS / WK / 16;
   constexpr int VPT = TN >= 64 ? TN / 64 : 1;  // vectors of 8 columns of dy a thread stages
@@ -259,25 +262,27 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   };
 
   // dy: this thread's vectors of 8 columns of the chunk, as they come; a row behind the last is the last one again (its partner
-  // in x is zero).  EDGE (the width is no multiple of 8): value by value, zeros behind the last column
-  constexpr int DW = P == 3 || EDGE ? 8 : 4, EB = P == 3 ? 4 : 2;  // words of a vector, bytes of a value
+  // in x is zero).  EDGE: 0 = the width is a multiple of 8; 1 = it is not: the vector that passes a row's end is the row's last 8
+  // values, shifted into place on their way to LDS; 2 = rows shorter than a vector: value by value, zeros behind the last column
+  constexpr int DW = P == 3 || EDGE == 2 ? 8 : 4, EB = P == 3 ? 4 : 2;  // words of a vector, bytes of a value
   uint32_t dyr[VPT][DW];
   const char *dyp[VPT];
   int dy_chunk = 0;
+  const int dy_co = co0 + tid % (TN / 8) * 8, dy_at = EDGE == 2 ? dy_co : (EDGE == 1 ? min(dy_co, p.cout - 8) : (dy_co < p.cout ? dy_co : 0));
+  const int dy_shift = min(dy_co - dy_at, 8);
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int i = tid + 512 * v, r = i / (TN / 8), co = co0 + i % (TN / 8) * 8;
+    const int i = tid + 512 * v, r = i / (TN / 8);
     const int row = r < rows_here ? r : rows_here - 1;
-    dyp[v] = (const char *)p.dy + ((int64_t)(chunk0 * WG8_ROWS + row) * p.dy_stride + (EDGE || co < p.cout ? co : 0)) * EB;
+    dyp[v] = (const char *)p.dy + ((int64_t)(chunk0 * WG8_ROWS + row) * p.dy_stride + dy_at) * EB;
   }
   auto load_dy = [&]() {  // of the next chunk, as often as it is called
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      if constexpr (EDGE) {
-        const int co = co0 + (tid + 512 * v) % (TN / 8) * 8;
+      if constexpr (EDGE == 2) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const char *src = dyp[v] + (co + j < p.cout ? j : p.cout - 1 - co) * EB;  // (columns behind the last: the last one)
+          const char *src = dyp[v] + (dy_co + j < p.cout ? j : p.cout - 1 - dy_co) * EB;  // (columns behind the last: the last one)
           if constexpr (P == 3) dyr[v][j] = *(const uint32_t *)src;
           else dyr[v][j] = *(const uint16_t *)src;
         }
@@ -304,6 +309,20 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       if (TN < 64 && r >= WG8_ROWS) continue;
       const uint32_t at = wg8_slot<TN>(r, cv);
       uint32_t w[P][4];
+      if constexpr (EDGE == 1 && P == 3) {
+#pragma unroll
+        for (int m = 1; m <= 8; m <<= 1)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dyr[v][j] = wg8_pick(dy_shift & m, j + m < 8 ? dyr[v][j + m < 8 ? j + m : 0] : 0u, dyr[v][j]);
+      } else if constexpr (EDGE == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          dyr[v][j] = wg8_pick(dy_shift & 1, __builtin_amdgcn_alignbit(j < 3 ? dyr[v][j < 3 ? j + 1 : 0] : 0u, dyr[v][j], 16), dyr[v][j]);
+#pragma unroll
+        for (int m = 1; m <= 4; m <<= 1)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dyr[v][j] = wg8_pick(dy_shift & 2 * m, j + m < 4 ? dyr[v][j + m < 4 ? j + m : 0] : 0u, dyr[v][j]);
+      }
       if constexpr (P == 3) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (EDGE) w[0][j] = dyr[v][2 * j] | dyr[v][2 * j + 1] << 16;
+          if constexpr (EDGE == 2) w[0][j] = dyr[v][2 * j] | dyr[v][2 * j + 1] << 16;
           else w[0][j] = dyr[v][j];
         }
       }
@@ -453,13 +472,15 @@ __global__ void __launch_bounds__(256) a8_fold_kernel(const float *__restrict__ 
 }
 
 // how a weight gradient is cut: columns of dy a block, units, row ranges
+// (bf16 rows whose width is no multiple of 8 keep to 128 columns: shifting needs registers that the tile of 256 has not.
+// [16000, 511] x [16000, 509]: 38 us, with 256 columns 51; f32 51 us.  Loaded value by value: 48, f32 69)
 struct Wg8Plan {
   int tn, kg, edge, units, groups, cotiles, chunks, per_split, splits;
 };
 #define WG8_UB 2
 static Wg8Plan wg8_plan(int64_t n_out, int kvol, int cin, int cout, int dtype, bool table) {
   Wg8Plan q;
-  q.edge = cout % 8 != 0;
+  q.edge = cout % 8 == 0 ? 0 : (cout >= 8 ? 1 : 2);
   q.tn = cout <= 32 ? 32 : (cout <= 64 ? 64 : (cout <= 128 || dtype == D3D_F32 || q.edge ? 128 : 256));
   q.units = (int)(((int64_t)kvol * ((cin + 7) / 8 * 8) + 63) / 64);
   q.kg = q.units <= 2 && !table ? 2 : 4;
@@ -535,17 +556,18 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
   } while (0)
 #define A8_WG_TN(F, P, EDGE)                                                                                                              \
   do {                                                                                                                                    \
-    if (q.tn == 32) A8_WG(F, P, 1, 4, 1, EDGE);                                                                                           \
+    if (q.edge == 2) A8_WG(F, P, 1, 4, 1, 2);                                                                                             \
+    else if (q.tn == 32) A8_WG(F, P, 1, 4, 1, EDGE);                                                                                      \
     else if (q.tn == 64) A8_WG(F, P, 2, 2, 1, EDGE);                                                                                      \
     else if (q.tn == 128) A8_WG(F, P, 4, 1, 1, EDGE);                                                                                     \
-    else if constexpr (P == 1 && !EDGE) A8_WG(F, P, 4, 1, 2, EDGE);                                                                       \
+    else if constexpr (P == 1 && !EDGE) A8_WG(F, P, 4, 1, 2, EDGE);                                                                      \
   } while (0)
 #define A8_WG_ALL(F)                                                                                                                      \
   do {                                                                                                                                    \
-    if (dtype == D3D_BF16 && !q.edge) A8_WG_TN(F, 1, false);                                                                              \
-    else if (dtype == D3D_BF16) A8_WG_TN(F, 1, true);                                                                                     \
-    else if (!q.edge) A8_WG_TN(F, 3, false);                                                                                              \
-    else A8_WG_TN(F, 3, true);                                                                                                            \
+    if (dtype == D3D_BF16 && !q.edge) A8_WG_TN(F, 1, 0);                                                                                  \
+    else if (dtype == D3D_BF16) A8_WG_TN(F, 1, 1);                                                                                        \
+    else if (!q.edge) A8_WG_TN(F, 3, 0);                                                                                                  \
+    else A8_WG_TN(F, 3, 1);                                                                                                               \
   } while (0)
   if (fmt == D3D_ACT8_INT8) A8_WG_ALL(D3D_ACT8_INT8);
   else A8_WG_ALL(D3D_ACT8_E4M3);

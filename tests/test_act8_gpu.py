@@ -234,6 +234,37 @@ def test_layouts_of_dy(act8, dtype):
         check_dw(act8.weight_grad(held, dy), restored(x, "int8"), dy, None)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cout", [2, 6, 9, 12, 15, 31, 33, 63, 65, 100, 127, 129, 257, 263])
+def test_widths_of_dy(act8, cout, dtype):
+    """widths that end inside a vector, with other values in front of the first row and behind the last, and between the rows"""
+    x = rows(150, 40, dtype, 1)
+    held = act8.hold(x, "int8")
+    big = torch.full((152, cout + 3), float("nan"), dtype=dtype, device="cuda")
+    big[1:151, 1:cout + 1] = rows(150, cout, dtype, 2)
+    check_dw(act8.weight_grad(held, big[1:151, 1:cout + 1]), restored(x, "int8"), big[1:151, 1:cout + 1], None)
+    nbr = table(150, 150, 5, 0.6, cout)
+    check_dw(act8.weight_grad(held, big[1:151, 1:cout + 1], nbr.cuda()), restored(x, "int8"), big[1:151, 1:cout + 1], nbr)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_non_finite_groups_reach_the_gradient(act8, dtype, fmt):
+    """a group that is restored as NaN makes NaN of its 32 channels, and of the offsets that meet its row only"""
+    x, dy = rows(70, 96, dtype, 1), rows(70, 33, dtype, 2)
+    dy[9].fill_(1.0)
+    x[9, 40], x[9, 95] = float("inf"), float("nan")
+    bad = torch.zeros(96, dtype=torch.bool)
+    bad[32:] = True
+    dw = act8.weight_grad(act8.hold(x, fmt), dy).cpu()
+    assert torch.isnan(dw[bad]).all() and torch.isfinite(dw[~bad]).all()
+    nbr = torch.arange(70).repeat(3, 1).int()
+    nbr[1][nbr[1] == 9] = -1  # (an absent neighbour)
+    dw = act8.weight_grad(act8.hold(x, fmt), dy, nbr.cuda()).cpu()
+    assert torch.isnan(dw[0][bad]).all() and torch.isnan(dw[2][bad]).all() and torch.isfinite(dw[1]).all()
+    assert torch.isfinite(dw[:, ~bad]).all()
+
+
 def test_non_finite_gradients_are_seen(act8):
     x, dy = rows(70, 64, torch.float32, 1), rows(70, 64, torch.float32, 2)
     dy[3, 5] = float("nan")

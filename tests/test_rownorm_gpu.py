@@ -253,7 +253,7 @@ def test_layouts(rn, dtype):
                            pre=rn.NormSpec("layer", leaf["pre_w"], leaf["pre_b"], 1e-5), gate=leaf["gate"], gate_act="sigmoid", scale=leaf["scale"])
             outs.append((h, z))
             grads.append(torch.autograd.grad((h, z), list(leaf.values()), (tt["dh"], tt["dz"])))
-        # (unaligned rows are read value by value and summed in another order: a few roundings apart)
+        # (unaligned rows are summed in another order: a few roundings apart)
         for a, b in zip(outs[0] + grads[0], outs[1] + grads[1]):
             assert (a - b).abs().max() <= (2 * HALF[dtype] + 1024 * EPS32) * max(1.0, float(b.detach().abs().max())), dtype
 

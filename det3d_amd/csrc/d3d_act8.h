@@ -183,6 +183,28 @@ template <bool BF16, int E> struct A8Row {
   }
 };
 
+// v combined over the T neighbouring lanes of a group, the same bits in every one of them (op commutes).  Steps of 1, 2, 4, 8 are
+// operand modifiers of the operation itself (lanes that agree already stand in for one another, so a mirrored row is a step),
+// 16 and 32 one instruction beside it: a dozen cycles a step, where a shuffle goes through LDS.
+template <int CTRL> __device__ __forceinline__ uint32_t a8_dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int T, class Op> __device__ __forceinline__ uint32_t a8_lanes(uint32_t v, Op op) {
+  if constexpr (T > 1) v = op(v, a8_dpp<0xb1>(v));   // 1 0 3 2
+  if constexpr (T > 2) v = op(v, a8_dpp<0x4e>(v));   // 2 3 0 1
+  if constexpr (T > 4) v = op(v, a8_dpp<0x141>(v));  // 8 lanes mirrored
+  if constexpr (T > 8) v = op(v, a8_dpp<0x140>(v));  // 16 lanes mirrored
+  if constexpr (T > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  if constexpr (T > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  return v;
+}
+
 // E values of a held row: LANES neighbouring lanes, each with E values, share a group (LANES * E = 32, or fewer where the
 // whole row is shorter)
 template <int FMT, int E, int LANES> struct A8Held {
@@ -195,11 +217,7 @@ template <int FMT, int E, int LANES> struct A8Held {
       const uint32_t u = __float_as_uint(v[j]) & 0x7fffffffu;
       top = u > top ? u : top;
     }
-#pragma unroll
-    for (int m = 1; m < LANES; m <<= 1) {
-      const uint32_t o = __shfl_xor(top, m, 64);
-      top = o > top ? o : top;
-    }
+    top = a8_lanes<LANES>(top, [](uint32_t l, uint32_t r) { return l > r ? l : r; });
     const uint32_t b = a8_scale_of<FMT>(top);
     const float down = a8_down(b);
     if (!inside) return;

@@ -16,10 +16,9 @@
 
 
 template <int T, int NT, int N> __device__ __forceinline__ void row_sum(float *v, float (&lds)[2][N][NT / 64], int &slot) {
+  const auto add = [](uint32_t l, uint32_t r) { return __float_as_uint(__uint_as_float(l) + __uint_as_float(r)); };
 #pragma unroll
-  for (int m = 1; m < (T < 64 ? T : 64); m <<= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], m, 64);
+  for (int k = 0; k < N; ++k) v[k] = __uint_as_float(a8_lanes<T < 64 ? T : 64>(__float_as_uint(v[k]), add));
   if constexpr (T > 64) {
     constexpr int W = T / 64;  // waves of a row
     const int wave = threadIdx.x >> 6, first = wave / W * W;
@@ -137,7 +136,7 @@ template <class S, int FMT> __global__ void __launch_bounds__(S::NT) row_join_fw
     rj_vector<S>(a.pre_bias, 0.f, 1.f, lane, c, qb);
   }
   for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
-    const bool mine = base + sub < a.n;
+    const bool mine = S::RPB == 1 || base + sub < a.n;
     const int64_t row = mine ? base + sub : a.n - 1;
     typename Row::Raw rx[NV], rf[NV], rg[NV];
     float ag = 1.f, dag;
@@ -248,8 +247,6 @@ __device__ __forceinline__ void rj_columns(const float *const *accs, int sums, i
   }
 }
 
-// the [c] vectors' length in LDS: whole vectors of either type
-__host__ __device__ static inline int rj_padded(int c) { return (c + 7) & ~7; }
 // E values of a [c] vector in LDS
 template <class S> __device__ __forceinline__ void rj_shared(const float *w, int at, float *v) {
 #pragma unroll
@@ -258,7 +255,8 @@ template <class S> __device__ __forceinline__ void rj_shared(const float *w, int
 
 // The backward pass keeps x, f, act and dH of a row in registers, five column sums over the rows beside them (40 registers of a
 // lane with 8 values), and the [c] vectors in LDS: with those in registers too it takes 180 of them, two waves to a SIMD in
-// place of four, and [8192, 4096] bf16 took 201 us in place of 169.
+// place of four, and [8192, 4096] bf16 took 201 us in
+// place of 169 (137 now: no lane branches around its part of the vectors, and the sums over lanes leave LDS alone).
 // HELD: 0 rows as they are, 1 + format: codes
 template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4 && S::NT < 512 ? 3 : 4) row_join_bwd_kernel(RjArgs p) {
   constexpr int E = S::E, T = S::T, NV = S::NV, EB = S::BF16 ? 2 : 4;
@@ -274,7 +272,8 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
   const D3dRowJoin &a = p.a;
   const D3dRowJoinGrads &g = p.g;
   const int lane = threadIdx.x & (T - 1), sub = threadIdx.x / T;
-  const int c = a.c, cp = rj_padded(c);
+  const int c = a.c;
+  constexpr int cp = T * S::EPL;  // the vectors' length in LDS: zeros behind the row's end, so that no lane needs a branch
   const bool has_f = HELD ? a.f_codes != nullptr : a.f != nullptr;
   float *const pw = vec, *const pb = vec + cp, *const sc = vec + 2 * cp, *const qw = vec + 3 * cp;
   for (int i = threadIdx.x; i < cp; i += S::NT) {
@@ -290,7 +289,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
   for (int j = 0; j < S::EPL; ++j) s_ef[j] = s_e[j] = s_qw[j] = s_qb[j] = 0.f;
 
   for (int64_t base = (int64_t)blockIdx.x * S::RPB; base < a.n; base += (int64_t)gridDim.x * S::RPB) {
-    const bool mine = base + sub < a.n;
+    const bool mine = S::RPB == 1 || base + sub < a.n;
     const int64_t row = mine ? base + sub : a.n - 1;
     // every load of the row first.  A row behind the last takes part in the sums over lanes with zero gradients
     typename In::Raw rx[NV], rf[NV];
@@ -342,7 +341,6 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           m[j] = ag;
-          w[j] = b[j] = s[j] = 0.f;
         }
         if (a.gate_cols > 1) {
           float unused;
@@ -352,11 +350,9 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
             for (int j = 0; j < E; ++j) rj_act<false>(a.gate_act, m[j], m[j], unused);
           }
         }
-        if (at < c) {
-          rj_shared<S>(pw, at, w);
-          rj_shared<S>(pb, at, b);
-          rj_shared<S>(sc, at, s);
-        }
+        rj_shared<S>(pw, at, w);
+        rj_shared<S>(pb, at, b);
+        rj_shared<S>(sc, at, s);
 #pragma unroll
         for (int j = 0; j < E; ++j)  // (behind the row's end everything is zero)
           h[k * E + j] = fmaf(s[j] * m[j], fmaf(f[k * E + j], w[j], b[j]), h[k * E + j]);
@@ -371,9 +367,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
         const int at = (k * T + lane) * E;
         float dz[E], w[E];
         Row::template open<ANY>(rdz[k], at, c, dz);
-#pragma unroll
-        for (int j = 0; j < E; ++j) w[j] = 0.f;
-        if (at < c) rj_shared<S>(qw, at, w);
+        rj_shared<S>(qw, at, w);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           const int q = k * E + j;
@@ -406,7 +400,7 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
       Row::template open<ANY>(rdh[k], at, c, dh);
       const bool in = at < c;
 #pragma unroll
-      for (int j = 0; j < E; ++j) d[k * E + j] = in ? d[k * E + j] + dh[j] : 0.f;
+      for (int j = 0; j < E; ++j) d[k * E + j] += dh[j];  // (behind the row's end the mean's share: the scale there is zero)
       if (g.dx && mine && in) Row::template put<ANY>((char *)g.dx + row * c * EB, at, c, d + k * E);
     }
     if (!has_f) continue;
@@ -419,7 +413,6 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
       for (int j = 0; j < E; ++j) {
         m[j] = ag;
         dm[j] = 1.f;
-        w[j] = b[j] = s[j] = 0.f;
       }
       if (a.gate_cols > 1) {  // (act(g) and act'(g) from the gate as it came: cheaper than to keep them)
         Row::template open<ANY>(rg[k], at, c, m);
@@ -428,11 +421,9 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
           for (int j = 0; j < E; ++j) rj_act<true>(a.gate_act, m[j], m[j], dm[j]);
         }
       }
-      if (at < c) {
-        rj_shared<S>(pw, at, w);
-        rj_shared<S>(pb, at, b);
-        rj_shared<S>(sc, at, s);
-      }
+      rj_shared<S>(pw, at, w);
+      rj_shared<S>(pb, at, b);
+      rj_shared<S>(sc, at, s);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int q = k * E + j;
@@ -643,9 +634,7 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
       p.part = g->ws;
     }
     const dim3 grid((unsigned)blocks), block(S::NT);
-    size_t lds = 4 * (size_t)rj_padded(a->c);
-    if (S::RPB > 1 && lds < (size_t)S::NT * S::EPL) lds = (size_t)S::NT * S::EPL;
-    lds *= sizeof(float);
+    const size_t lds = (S::RPB > 4 ? S::RPB : 4) * (size_t)S::T * S::EPL * sizeof(float);
     const void *fn = held == 0 ? (const void *)row_join_bwd_kernel<S, 0>
                                : (held == 1 ? (const void *)row_join_bwd_kernel<S, 1> : (const void *)row_join_bwd_kernel<S, 2>);
     if (lds > 48 * 1024) D3D_HIP_TRY(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));

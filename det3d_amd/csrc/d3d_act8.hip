@@ -149,15 +149,12 @@ template <int FMT> __device__ __forceinline__ uint4 wg8_restore(uint2 w, uint32_
   // 8 codes to bf16: exact
   const float s = a8_up(b);
   if constexpr (FMT == D3D_ACT8_INT8) {
-    // biased to unsigned bytes, whose conversion is one instruction: (code + 128) 2^s - 128 2^s; the upper halves of the f32
-    // values are their bf16
-    const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u;
-    const float m = -128.f * s;
+    // a signed byte's conversion is one instruction, scaling another (exact); the upper halves of the f32 values are their bf16
     uint32_t v[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = __float_as_uint(fmaf((float)((x >> (8 * j)) & 0xffu), s, m));
-      v[4 + j] = __float_as_uint(fmaf((float)((y >> (8 * j)) & 0xffu), s, m));
+      v[j] = __float_as_uint((float)((int)(w.x << (24 - 8 * j)) >> 24) * s);
+      v[4 + j] = __float_as_uint((float)((int)(w.y << (24 - 8 * j)) >> 24) * s);
     }
     return make_uint4(__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u),
                       __builtin_amdgcn_perm(v[5], v[4], 0x07060302u), __builtin_amdgcn_perm(v[7], v[6], 0x07060302u));

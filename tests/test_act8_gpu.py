@@ -265,6 +265,20 @@ def test_non_finite_groups_reach_the_gradient(act8, dtype, fmt):
     assert torch.isfinite(dw[:, ~bad]).all()
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_largest_and_smallest_rows_through_the_gradient(act8, dtype, fmt):
+    """groups at both ends of the scales' range: a restored value is finite and meets dy as it is"""
+    x, dy = rows(130, 64, dtype, 1), rows(130, 16, dtype, 2)
+    x = x / x.abs().amax()
+    x[:65, :32] *= 3.3e38
+    x[65:, 32:] *= 1e-28
+    dy[:65] *= 1e-25
+    held = act8.hold(x, fmt)
+    assert torch.isfinite(held.restore()).all()
+    check_dw(act8.weight_grad(held, dy), restored(x, fmt), dy, None)
+
+
 def test_non_finite_gradients_are_seen(act8):
     x, dy = rows(70, 64, torch.float32, 1), rows(70, 64, torch.float32, 2)
     dy[3, 5] = float("nan")
@@ -300,6 +314,22 @@ def test_on_another_stream_and_in_a_graph(act8):
         g1.replay()
         torch.cuda.synchronize()
         assert torch.equal(a, want) and torch.equal(b, want)
+
+
+def test_two_at_once(act8):
+    """the same held rows read on two streams at the same time, each call with a workspace of its own"""
+    x, dy = rows(3000, 64, torch.float32, 1), [rows(3000, 64, torch.float32, 2 + k) for k in range(2)]
+    held, nbr = act8.hold(x), table(3000, 3000, 27, 0.5, 1).cuda()
+    want = [act8.weight_grad(held, d, nbr) for d in dy]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(act8.weight_grad(held, dy[k], nbr))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[k]) for k in range(2) for g in got[k])
 
 
 def test_refusals(act8):

@@ -332,6 +332,36 @@ def test_in_a_graph_and_on_another_stream(rn, checkpoint):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("c,dtype", [(4096, torch.bfloat16), (8192, torch.bfloat16), (8192, torch.float32), (4093, torch.bfloat16)])
+def test_wide_rows_in_a_graph_and_two_at_once(rn, c, dtype):
+    """rows whose [c] vectors take most of a CU's LDS: a first call that is captured, and two streams at the same time"""
+    t = make(21, c, dtype, "full")
+    leaf = {k: t[k].clone().requires_grad_() for k in LEAVES}
+
+    def step():
+        h, z = rn.join(leaf["x"], leaf["f"], post=rn.NormSpec("rms", leaf["post_w"], leaf["post_b"], 1e-5),
+                       pre=rn.NormSpec("layer", leaf["pre_w"], leaf["pre_b"], 1e-5), gate=leaf["gate"], gate_act="silu",
+                       scale=leaf["scale"], checkpoint="e4m3")
+        return (h.detach(), z.detach()) + torch.autograd.grad((h, z), list(leaf.values()), (t["dh"], t["dz"]))
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    want = step()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    both = [[], []]
+    for _ in range(3):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                both[k].append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for k in range(2) for r in both[k] for a, b in zip(r, want))
+
+
 def test_refusals(rn):
     from det3d_amd._lib import D3dError
 

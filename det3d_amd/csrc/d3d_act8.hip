@@ -453,19 +453,31 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   }
 }
 
-// the row ranges' sums in their order: four parts of the ranges side by side, then the parts
-__global__ void __launch_bounds__(256) a8_fold_kernel(const float *__restrict__ part, int64_t count, int splits, float *__restrict__ out) {
-  __shared__ float sum[4][64];
+// the row ranges' sums in their order: PARTS parts of the ranges side by side, then the parts.  Bound by latency where there are
+// many ranges and few weights ([27, 16, 16], 128 ranges: 9.8 us with 4 parts, 3.9 with 16; [27, 64, 64], 36 ranges: 4.8 and 7.1),
+// by HBM where there are few and many (4 MB of weights, 16 ranges: 10.6 us; 15.9 with one load of a thread in flight)
+template <int PARTS>
+__global__ void __launch_bounds__(64 * PARTS) a8_fold_kernel(const float *__restrict__ part, int64_t count, int splits, float *__restrict__ out) {
+  __shared__ float sum[PARTS][64];
   const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int q = threadIdx.x >> 6, per = (splits + 3) / 4;
+  const int q = threadIdx.x >> 6, per = (splits + PARTS - 1) / PARTS;
   float s = 0.f;
   if (i < count) {
     const int last = (q + 1) * per < splits ? (q + 1) * per : splits;
+#pragma unroll 4
     for (int k = q * per; k < last; ++k) s += part[k * count + i];
   }
   sum[q][threadIdx.x & 63] = s;
   __syncthreads();
-  if (q == 0 && i < count) out[i] = (s + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
+  if (q != 0 || i >= count) return;
+  float t[PARTS];
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) t[k] = sum[k][threadIdx.x];
+#pragma unroll
+  for (int m = 1; m < PARTS; m <<= 1)
+#pragma unroll
+    for (int k = 0; k < PARTS; k += 2 * m) t[k] += t[k + m];
+  out[i] = t[0];
 }
 
 // how a weight gradient is cut: columns of dy a block, units, row ranges
@@ -573,8 +585,9 @@ extern "C" int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int f
 #undef A8_WG
   D3D_LAUNCH_TRY("a8_wgrad_kernel");
   if (q.splits > 1) {
-    hipLaunchKernelGGL(a8_fold_kernel, dim3((unsigned)((p.count + 63) / 64)), dim3(256), 0, stream, (const float *)workspace, p.count,
-                       q.splits, dw);
+    const dim3 columns((unsigned)((p.count + 63) / 64));
+    if (q.splits > 32 && columns.x <= 256) hipLaunchKernelGGL(a8_fold_kernel<16>, columns, dim3(1024), 0, stream, (const float *)workspace, p.count, q.splits, dw);
+    else hipLaunchKernelGGL(a8_fold_kernel<4>, columns, dim3(256), 0, stream, (const float *)workspace, p.count, q.splits, dw);
     D3D_LAUNCH_TRY("a8_fold_kernel");
   }
   return D3D_OK;

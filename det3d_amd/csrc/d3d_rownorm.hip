@@ -6,10 +6,14 @@
 //   norm^T    with xhat = (x - mu) r and d = w dy:  r (d - mean(d) - xhat mean(d xhat));  rms has no mu and no mean(d)
 //
 // Bound by HBM: a few dozen f32 operations a value against 8 to 40 bytes.  So one pass: T lanes own a row and keep it in
-// registers (NV vectors of E values a lane) from the first load to the last store; the sums of a row go over the T lanes, by
-// shuffles up to a wave, through LDS beyond it.  The variance is a second sum over the registers, around the mean that the
+// registers (NV vectors of E values a lane) from the first load to the last store; the sums of a row go over the T lanes, in
+// registers up to a wave, through LDS beyond it.  The variance is a second sum over the registers, around the mean that the
 // first gave: no cancellation.  The backward pass recomputes u, h and their statistics from x and f (or from their 8-bit
 // codes) instead of reading saved ones.
+//
+// Join of [8192, 4096] bf16 with both norms, a full gate and e4m3 rows: forward 78 us (404 MB, 5.2 TB/s), backward 137 us (471 MB,
+// 3.4 TB/s: about 750 vector instructions a row and wave, the issue of the SIMDs is two thirds of it), fold 8 us.  Norm of
+// [60013, 128] f32 with int8 rows: forward 17 us, backward 15 us (70 MB each), fold 5 us.
 #include "d3d_act8.h"
 #include <string.h>
 #include <type_traits>
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(1024) row_join_fold_kernel(const float *__rest
   float t0 = 0.f, t1 = 0.f;
   if (i < c) {
     const float *src = part + (int64_t)pair * 2 * c + i;
-#pragma unroll 4
+#pragma unroll 8
     for (int b = y; b < blocks; b += 32) {
       t0 += src[b * step];
       t1 += src[b * step + c];
@@ -504,9 +508,12 @@ __global__ void __launch_bounds__(1024) row_join_fold_kernel(const float *__rest
 }
 
 #define RJ_MAXC 8192
+// blocks of the backward pass: at most four waves to a SIMD, and behind the first 256 blocks two row groups to a block, since every
+// block writes its column sums and the fold reads them ([2057, 333] f32: 15.1 + 5.2 us, with one row group 14.6 + 7.8)
 static int rj_blocks_bwd(int64_t n, int rpb, int nt) {
-  const int64_t nb = (n + rpb - 1) / rpb, most = 256 * (1024 / nt);  // (four waves to a SIMD)
-  return (int)(nb > most ? most : nb);
+  const int64_t nb = (n + rpb - 1) / rpb, most = 256 * (1024 / nt);
+  const int64_t two = nb > 512 ? (nb + 1) / 2 : (nb > 256 ? 256 : nb);
+  return (int)(two > most ? most : two);
 }
 
 static int rj_check(const D3dRowJoin *a, bool backward, const char *who) {

@@ -448,13 +448,19 @@ def launch_dgrad(rb, gout, wd, cout, pad_cin, gin, ep, stream):
 
 
 # --------------------------------------------------------------------- autograd
+def _kept_format():
+    """the 8-bit format that rows are kept in for a backward pass, None if there will be none or it reads full rows"""
+    return _runtime.held_format() if torch.is_grad_enabled() else None
+
+
 class _SparseConvFn(torch.autograd.Function):
     @staticmethod
     @_lib.ctx_forward
-    def forward(ctx, feats, weight, bias, rb, stats, link):
+    def forward(ctx, feats, weight, bias, rb, stats, link, held):
         """stats: epilogue_ws() buffer or None -- the launch leaves sum / sum-of-squares of its output rows (the
         batch statistics of the BatchNorm that follows) in stats[:2*cout].  link: _BnLink of the fused BN(+ReLU)
-        that produced `feats`, or None -- the backward's dgrad launch then also reduces that BN's gradient sums."""
+        that produced `feats`, or None -- the backward's dgrad launch then also reduces that BN's gradient sums.
+        held: the 8-bit format that `feats` is kept in for the backward (_kept_format), or None."""
         _need_cuda(feats, "sparse conv")
         L = _lib.lib()
         if feats.dtype not in _DT:
@@ -486,12 +492,11 @@ class _SparseConvFn(torch.autograd.Function):
         rc = launch_fwd(rb, feats, wpack, b, pad_cin, cout, out, ep, _lib.stream_ptr(feats.device))
         _lib.check(rc, "d3d_sparse_conv_fwd")
         ctx.stats_done = ep is not None
-        fmt = _runtime.held_format()
         ctx.feat_dtype, ctx.held = feats.dtype, None
-        if fmt is not None and ctx.needs_input_grad[1]:  # the weight gradient alone reads the input rows: keep them in 8 bits
-            held = act8.hold(feats, fmt)
-            ctx.save_for_backward(held.buf, weight)
-            ctx.held = held.meta()
+        if held is not None and ctx.needs_input_grad[1]:  # the weight gradient alone reads the input rows: keep them in 8 bits
+            rows = act8.hold(feats, held)
+            ctx.save_for_backward(rows.buf, weight)
+            ctx.held = rows.meta()
         else:
             ctx.save_for_backward(feats, weight)
         ctx.wd = wd
@@ -558,7 +563,7 @@ class _SparseConvFn(torch.autograd.Function):
             gw = gw.reshape(weight.shape).to(weight.dtype)
         if ctx.has_bias and ctx.needs_input_grad[2]:
             gb = gout.float().sum(0)
-        return gin, gw, gb, None, None, None
+        return gin, gw, gb, None, None, None, None
 
 
 class _BNReLUFn(torch.autograd.Function):
@@ -568,7 +573,7 @@ class _BNReLUFn(torch.autograd.Function):
 
     @staticmethod
     @_lib.ctx_forward
-    def forward(ctx, x, weight, bias, running_mean, running_var, momentum, eps, training, relu, stats, link):
+    def forward(ctx, x, weight, bias, running_mean, running_var, momentum, eps, training, relu, stats, link, held):
         L = _lib.lib()
         x = x.contiguous()
         n, c = x.shape
@@ -587,11 +592,11 @@ class _BNReLUFn(torch.autograd.Function):
                             save[0].data_ptr(), save[1].data_ptr(), st)
         _lib.check(rc, "d3d_bn_apply")
         # in 8 bits the backward sweeps read the restored rows (with the statistics of the full ones)
-        fmt, ctx.held = _runtime.held_format(), None
-        if fmt is not None and training and link is None and any(ctx.needs_input_grad[:3]):
-            held = act8.hold(x, fmt)
-            ctx.save_for_backward(held.buf, weight, bias, save)
-            ctx.held = held.meta()
+        ctx.held = None
+        if held is not None and training and link is None and any(ctx.needs_input_grad[:3]):
+            rows = act8.hold(x, held)
+            ctx.save_for_backward(rows.buf, weight, bias, save)
+            ctx.held = rows.meta()
         else:
             ctx.save_for_backward(x, weight, bias, save)
         ctx.relu = relu
@@ -639,7 +644,7 @@ class _BNReLUFn(torch.autograd.Function):
             link.reduced = False  # a second backward over the same graph runs its own reduction sweep
         gw = g[0].to(weight.dtype) if weight is not None else None
         gb = g[1].to(bias.dtype) if bias is not None else None
-        return dx, gw, gb, None, None, None, None, None, None, None, None
+        return dx, gw, gb, None, None, None, None, None, None, None, None, None
 
 
 def _fusable_bn(bn, feats, channels=None):
@@ -666,7 +671,7 @@ def bn_relu(bn, feats, relu, stats=None, link=None):
     """apply `bn` (an nn.BatchNorm1d) and optionally ReLU to sparse features with the fused HIP
     kernels; state (running stats) lives in the module exactly as with F.batch_norm."""
     return _BNReLUFn.apply(feats, bn.weight, bn.bias, bn.running_mean, bn.running_var,
-                           bn.momentum, bn.eps, bn.training, relu, stats, link)
+                           bn.momentum, bn.eps, bn.training, relu, stats, link, _kept_format())
 
 
 def conv_bn_relu(conv, bn, relu, x, link_in=None, want_link=False):
@@ -706,7 +711,7 @@ def bn_relu_2d(bn, x, relu):
     b, c, h, w = x.shape
     rows = x.permute(0, 2, 3, 1).reshape(b * h * w, c)  # a view: channels-last memory is [B,H,W,C]
     y = _BNReLUFn.apply(rows, bn.weight, bn.bias, bn.running_mean, bn.running_var, bn.momentum, bn.eps,
-                        bn.training, relu, None, None)
+                        bn.training, relu, None, None, None)
     # like bn_relu(): num_batches_tracked is not advanced (one launch per layer for a counter that
     # momentum-based running statistics never read)
     return y.view(b, h, w, c).permute(0, 3, 1, 2)
@@ -867,7 +872,7 @@ class SparseConvolution(SparseModule):
                 stats = None  # no MFMA tiling for this channel pair: the BatchNorm runs its own statistics sweep
             elif stats is True:
                 stats = epilogue_ws(x.features.device, rb.n_out, self.out_channels)
-        out_feats = _SparseConvFn.apply(x.features, self.weight, self.bias, rb, stats, link)
+        out_feats = _SparseConvFn.apply(x.features, self.weight, self.bias, rb, stats, link, _kept_format())
         out = SparseConvTensor(out_feats, rb.out_indices if not self.subm else x.indices,
                                self.out_spatial_shape(x.spatial_shape), x.batch_size, x.grid)
         out.indice_dict = x.indice_dict

@@ -95,6 +95,25 @@ def test_a_batch_norm_sweep_reads_its_held_rows(dtype):
     assert ((dx.double() - want).abs() <= 1000 * 2.0 ** -24 * mag + slack + half * want.abs())[clear].all()
 
 
+def test_nothing_is_held_without_a_backward_pass(monkeypatch):
+    """a model that answers does not pay for the checkpoint, and dense maps keep full rows"""
+    from det3d_amd import act8, runtime, spconv
+
+    conv = spconv.SubMConv3d(16, 32, 3, indice_key="a").cuda()
+    bn = nn.BatchNorm1d(32, eps=1e-3, momentum=0.01).cuda().train()
+    bn2d = nn.BatchNorm2d(32, eps=1e-3, momentum=0.01).cuda().train()
+    runtime.configure(activations="int8")
+    calls = []
+    hold = act8.hold
+    monkeypatch.setattr(act8, "hold", lambda *a, **k: calls.append(1) or hold(*a, **k))
+    with torch.no_grad():
+        want = spconv.bn_relu(bn, conv(sites()()).features, True)
+    assert not calls
+    assert torch.equal(spconv.bn_relu(bn, conv(sites()()).features, True), want) and len(calls) == 2
+    spconv.bn_relu_2d(bn2d, torch.randn(2, 32, 8, 8, device="cuda").contiguous(memory_format=torch.channels_last).requires_grad_(), True)
+    assert len(calls) == 2
+
+
 def _backbone(norm_cfg=None, seed=0):
     from det3d_amd.backbones import SpMiddleResNetFHD
 

@@ -104,19 +104,40 @@ def _call(x, f, post, pre, gate, gate_act, alpha, checkpoint):
 
 
 def _forward(call, x, f, gate, scale, post, pre, arena, hx=None, hf=None):
+    """(outputs, the launch's description; None of no rows)"""
     n, c, dev = call.n, call.c, call.dev
     h = mem.empty((n, c), call.dtype, dev, arena) if f is not None else None
     z = mem.empty((n, c), call.dtype, dev, arena) if call.pre[0] else None
+    d = None
     if n:
         d = call.desc(x, f, gate, scale, post, pre, h, z, hx, hf)
         act8.launch("d3d_row_join_fwd", dev, _lib.lib().d3d_row_join_fwd, ctypes.byref(d))
     if f is None:
-        return z
-    return h if z is None else (h, z)
+        return z, d
+    return (h if z is None else (h, z)), d
+
+
+def _addresses(tensors):
+    return [None if t is None else t.data_ptr() for t in tensors]
+
+
+def _gradient(t, dtype, c):
+    """(an output's gradient as rows, its address and row stride)"""
+    if t is None:
+        return None, None, 0
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    if t.is_contiguous():
+        return t, t.data_ptr(), c
+    t = act8.rows_of(t, "rownorm")
+    return t, t.data_ptr(), act8.row_stride(t)
 
 
 class _JoinFn(torch.autograd.Function):
-    """both operators (f None: the norm alone); the weights travel as tensors of their own so that autograd sees them"""
+    """both operators (f None: the norm alone); the weights travel as tensors of their own so that autograd sees them.
+
+    What the backward pass can know in advance is prepared in the forward pass: autograd runs the former on a thread of its own,
+    whose first instructions after a wait are several times slower."""
 
     @staticmethod
     def forward(ctx, call, x, f, gate, scale, post_w, post_b, pre_w, pre_b):
@@ -125,13 +146,22 @@ class _JoinFn(torch.autograd.Function):
         if call.fmt is not None:
             hx = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease)
             hf = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease) if f is not None else None
-        out = _forward(call, x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), lease.arena, hx, hf)
+        out, d = _forward(call, x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), lease.arena, hx, hf)
         ctx.set_materialize_grads(False)
         ctx.call, ctx.lease = call, lease
         # (in 8 bits the backward pass reads the codes alone: x and f are free once nobody else holds them)
         if hx is not None:
             x, f = hx.buf, hf.buf if hf is not None else None
-        ctx.save_for_backward(x, f, gate, scale, post_w, post_b, pre_w, pre_b)
+        saved = (x, f, gate, scale, post_w, post_b, pre_w, pre_b)
+        ctx.save_for_backward(*saved)
+        _, _, _, _, need_s, need_pw, need_pb, need_qw, need_qb = ctx.needs_input_grad
+        ctx.count = need_s + need_pw + need_pb + need_qw + need_qb
+        ctx.floats = _lib.lib().d3d_row_join_ws_floats(call.n, call.c, call.dt, ctx.count) if ctx.count and call.n else 0
+        if d is not None:
+            d.h = d.z = None
+            if hx is not None:
+                d.x = d.f = None
+        ctx.desc, ctx.at = d, _addresses(saved)
         return out
 
     @staticmethod
@@ -141,7 +171,7 @@ class _JoinFn(torch.autograd.Function):
         call = ctx.call
         n, c, dev, dtype = call.n, call.c, call.dev, call.dtype
         arena = ctx.lease.check("rownorm")
-        x, f, gate, scale, post_w, post_b, pre_w, pre_b = ctx.saved_tensors
+        saved = ctx.saved_tensors
         dh = dz = None
         if call.has_f:
             dh = grads[0]
@@ -151,49 +181,39 @@ class _JoinFn(torch.autograd.Function):
             dz = grads[0]
         if dh is None and dz is None:
             return (None,) * 9
-        if dh is not None:
-            dh = act8.rows_of(dh if dh.dtype == dtype else dh.to(dtype), "rownorm")
-        if dz is not None:
-            dz = act8.rows_of(dz if dz.dtype == dtype else dz.to(dtype), "rownorm")
-        hx = hf = None
-        if call.fmt is not None:
-            hx = act8.Held(x, (n, c), dtype, call.fmt, ctx.lease)
-            hf = act8.Held(f, (n, c), dtype, call.fmt, ctx.lease) if f is not None else None
-            x = f = None
+        dh, dh_at, dh_stride = _gradient(dh, dtype, c)
+        dz, dz_at, dz_stride = _gradient(dz, dtype, c)
         _, need_x, need_f, need_g, need_s, need_pw, need_pb, need_qw, need_qb = ctx.needs_input_grad
         dx = mem.empty((n, c), dtype, dev, arena) if need_x else None
         df = mem.empty((n, c), dtype, dev, arena) if need_f else None
         dgate = mem.empty((n, call.gate_cols), dtype, dev, arena) if need_g else None
         # scale, post weight, post bias, pre weight, pre bias: those that are asked for, each a row of one buffer
-        count = need_s + need_pw + need_pb + need_qw + need_qb
-        ds = dpw = dpb = dqw = dqb = None
-        if count:
-            sums = torch.empty((count, c), dtype=torch.float32, device=dev)
-            rows = sums.unbind(0)
-            at = 0
-            if need_s:
-                ds, at = rows[0], 1
-            if need_pw:
-                dpw, at = rows[at], at + 1
-            if need_pb:
-                dpb, at = rows[at], at + 1
-            if need_qw:
-                dqw, at = rows[at], at + 1
-            if need_qb:
-                dqb = rows[at]
+        sums = [None] * 5
+        if ctx.count:
+            buf = torch.empty((ctx.count, c), dtype=torch.float32, device=dev)
+            rows = iter(buf.unbind(0))
+            sums = [next(rows) if need else None for need in (need_s, need_pw, need_pb, need_qw, need_qb)]
         if n:
-            L = _lib.lib()
-            ws, floats = None, 0
-            if count:
-                floats = L.d3d_row_join_ws_floats(n, c, call.dt, count)
-                ws = mem.empty((floats,), torch.float32, dev, arena)
-            d = call.desc(x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), None, None, hx, hf)
-            g = _lib.RowJoinGrads(*_rows(dh), *_rows(dz), _dp(dx), _dp(df), _dp(dgate), _dp(ds), _dp(dpw), _dp(dpb), _dp(dqw), _dp(dqb),
-                                  _dp(ws), floats)
-            act8.launch("d3d_row_join_bwd", dev, L.d3d_row_join_bwd, ctypes.byref(d), ctypes.byref(g))
-        elif count:
-            sums.zero_()
-        return None, dx, df, dgate, ds, dpw, dpb, dqw, dqb
+            d = ctx.desc
+            if _addresses(saved) != ctx.at:  # (saved tensors come back elsewhere: hooks that pack them)
+                d = _elsewhere(call, ctx.lease, saved)
+            ws = mem.empty((ctx.floats,), torch.float32, dev, arena) if ctx.count else None
+            g = _lib.RowJoinGrads(dh_at, dh_stride, dz_at, dz_stride, _dp(dx), _dp(df), _dp(dgate), *_addresses(sums), _dp(ws), ctx.floats)
+            act8.launch("d3d_row_join_bwd", dev, _lib.lib().d3d_row_join_bwd, ctypes.byref(d), ctypes.byref(g))
+        elif ctx.count:
+            buf.zero_()
+        return (None, dx, df, dgate, *sums)
+
+
+def _elsewhere(call, lease, saved):
+    """the backward pass's description with the saved tensors where they are now"""
+    x, f, gate, scale, post_w, post_b, pre_w, pre_b = saved
+    hx = hf = None
+    if call.fmt is not None:
+        hx = act8.Held(x, (call.n, call.c), call.dtype, call.fmt, lease)
+        hf = act8.Held(f, (call.n, call.c), call.dtype, call.fmt, lease) if f is not None else None
+        x = f = None
+    return call.desc(x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), None, None, hx, hf)
 
 
 def _apply(call, x, f, gate, scale):
@@ -203,7 +223,7 @@ def _apply(call, x, f, gate, scale):
         for t in (x, f, gate, scale, pw, pb, qw, qb):
             if t is not None and t.requires_grad:
                 return _JoinFn.apply(call, x, f, gate, scale, pw, pb, qw, qb)
-    return _forward(call, x, f, gate, scale, (pw, pb), (qw, qb), None)
+    return _forward(call, x, f, gate, scale, (pw, pb), (qw, qb), None)[0]
 
 
 def norm(x, spec, checkpoint=None):

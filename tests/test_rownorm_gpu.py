@@ -332,6 +332,26 @@ def test_in_a_graph_and_on_another_stream(rn, checkpoint):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_saved_tensors_that_were_packed_away(rn, checkpoint):
+    """hooks that move what is saved for the backward pass (to the host and back): the same gradients"""
+    t = make(300, 72, torch.float32, "row")
+    leaf = {k: t[k].clone().requires_grad_() for k in LEAVES}
+
+    def step():
+        h, z = rn.join(leaf["x"] * 1.0, leaf["f"] * 1.0, post=rn.NormSpec("rms", leaf["post_w"], leaf["post_b"], 1e-5),
+                       pre=rn.NormSpec("layer", leaf["pre_w"], leaf["pre_b"], 1e-5), gate=leaf["gate"], gate_act="silu",
+                       scale=leaf["scale"], checkpoint=checkpoint)
+        return lambda: torch.autograd.grad((h, z), list(leaf.values()), (t["dh"], t["dz"]))
+
+    want = step()()
+    with torch.autograd.graph.save_on_cpu():
+        later = step()
+    keep = [torch.full((300, 72), float("nan"), device="cuda") for _ in range(8)]  # (where the packed tensors lay)
+    got = later()
+    assert len(keep) == 8 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("c,dtype", [(4096, torch.bfloat16), (8192, torch.bfloat16), (8192, torch.float32), (4093, torch.bfloat16)])
 def test_wide_rows_in_a_graph_and_two_at_once(rn, c, dtype):
     """rows whose [c] vectors take most of a CU's LDS: a first call that is captured, and two streams at the same time"""

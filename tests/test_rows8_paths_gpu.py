@@ -225,6 +225,23 @@ def test_a_backbone_with_row_norms_trains(kind, mode):
         assert torch.allclose(model(*args), out, rtol=1e-4, atol=1e-4 * float(out.abs().max()))  # nothing depends on the mode
 
 
+@pytest.mark.parametrize("norm_cfg", [None, dict(type="RMS", eps=1e-3)])
+def test_a_backbone_on_held_rows_under_autocast(norm_cfg):
+    """bfloat16 features all the way: finite gradients of the parameters' type, an output within a bfloat16 pass of the float32 one"""
+    from det3d_amd import runtime
+
+    runtime.configure(activations="int8")
+    model, args = _backbone(norm_cfg), _voxels()
+    with torch.no_grad():
+        full = model(*args)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out, grads = _step(model, args)
+    assert out.dtype == torch.bfloat16
+    assert all(torch.isfinite(g).all() and g.dtype == p.dtype for g, p in zip(grads, model.parameters()))
+    # some 25 layers round their rows to half a step of bfloat16 each, products of them once more: 50 * 2^-8 of the norm at most
+    assert float((out.float() - full).norm()) <= 50 * 2.0 ** -8 * float(full.norm())
+
+
 def test_maps_and_pillars_take_row_norms():
     from det3d_amd.nn_utils import build_norm_layer
 

@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
 
   // dy: this thread's vectors of 8 columns of the chunk, as they come; a row behind the last is the last one again (its partner
   // in x is zero).  EDGE: 0 = the width is a multiple of 8; 1 = it is not: the vector that passes a row's end is the row's last 8
-  // values, shifted into place on their way to LDS; 2 = rows shorter than a vector: value by value, zeros behind the last column
+  // values, shifted into place on their way to LDS; 2 = rows shorter than a vector: value by value, the last one again behind it
+  // (what stands in columns behind the last is multiplied and not stored)
   constexpr int DW = P == 3 || EDGE == 2 ? 8 : 4, EB = P == 3 ? 4 : 2;  // words of a vector, bytes of a value
   uint32_t dyr[VPT][DW];
   const char *dyp[VPT];
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       if constexpr (EDGE == 2) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const char *src = dyp[v] + (dy_co + j < p.cout ? j : p.cout - 1 - dy_co) * EB;  // (columns behind the last: the last one)
+          const char *src = dyp[v] + (dy_co + j < p.cout ? j : p.cout - 1 - dy_co) * EB;
           if constexpr (P == 3) dyr[v][j] = *(const uint32_t *)src;
           else dyr[v][j] = *(const uint16_t *)src;
         }

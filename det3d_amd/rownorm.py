@@ -14,7 +14,9 @@ None: a factor 1; scale None: alpha alone; pre None: only h comes back.
 gradients are then those at the restored rows: exactly what the backward pass of `join(restored x, restored f, ...)` gives.
 
 Sums over a row and over the rows (gradients of weights, biases and scales) are float32 in a fixed order: two identical calls
-give the same bits.  `RowNorm` is the module: `norm_cfg = dict(type="RMS" | "LN")` of the backbones and necks builds it
+give the same bits.  Both directions can be captured into a graph; as with any autograd node, an eager graph of the same leaves must
+not be alive then (a leaf's node belongs to the stream of the first graph that holds it, and the capture would draw that stream in).
+`RowNorm` is the module: `norm_cfg = dict(type="RMS" | "LN")` of the backbones and necks builds it
 (nn_utils.build_norm_layer), and SparseBasicBlock joins its identity branch through it.
 """
 import collections

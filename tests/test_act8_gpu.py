@@ -64,6 +64,7 @@ def test_restored_values_are_the_definition(act8, n, c, dtype, fmt):
     x = rows(n, c, dtype, n * 1000 + c)
     held = act8.hold(x, fmt)
     assert held.codes.shape == (n, act8.pitch(c)) and held.scales.shape == (n, act8.pitch(c) // 32)
+    assert held.nbytes() == held.codes.numel() + held.scales.numel()
     want = restored(x, fmt)
     for out_type in DTYPES:  # exact in either type
         got = held.restore(out_type)

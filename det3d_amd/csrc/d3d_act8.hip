@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   // Staging.  A thread owns one row of the chunk and 8 columns of each unit.  Loads stay in flight only while nothing touches
   // their registers: no select behind them, no branch around them.  What is absent (a row or a column behind the last, a table
   // entry out of range) reads beyond the buffer, which gives zeros: the scale 0 makes the row add nothing, whatever dy has there.
+  // The range check takes in the vector offset alone: everything that moves is part of it, and the scalar offset is 0.
   // Offsets are 32 bits: the table and the codes behind one stay below 2^31 bytes and 2^24 rows (checked on the host); without a
   // table the base moves with the chunk.
   const int srow = tid >> 3, sseg = tid & 7;
@@ -239,8 +240,13 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   uint2 code[KG];
   uint32_t sc[KG];
   const __amdgpu_buffer_rsrc_t tab_rs = __builtin_amdgcn_make_buffer_rsrc((void *)p.nbr, 0, TABLE ? p.tab_bytes : 0, 0x00020000);
-  auto load_idx = [&](int u, int chunk) {  // (rows behind the last read other entries, or zeros: load_code knows)
-    if constexpr (TABLE) idx[u] = __builtin_amdgcn_raw_buffer_load_b32(tab_rs, (int)tab_off[u], chunk * (WG8_ROWS * 4), 0);
+  // of the next chunk, as often as it is called: up to two chunks behind the last.  Rows behind the last read entries of other
+  // offsets, which load_code drops, and behind the table's end zeros: an offset is below its 2^31 bytes and four chunks
+  auto load_idx = [&](int u) {
+    if constexpr (TABLE) {
+      idx[u] = __builtin_amdgcn_raw_buffer_load_b32(tab_rs, (int)tab_off[u], 0, 0);
+      tab_off[u] += WG8_ROWS * 4u;
+    }
   };
   auto load_code = [&](int u, int chunk) {
     bool in = chunk < lim[u];
@@ -351,19 +357,19 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
       for (int r = 0; r < 16; ++r) acc[u][n][r] = 0.f;
 
 #pragma unroll
-  for (int u = 0; u < KG; ++u) load_idx(u, 0);
+  for (int u = 0; u < KG; ++u) load_idx(u);
   load_dy();
   __builtin_amdgcn_sched_barrier(0);  // (in this order, as in the loop: the waits at its top count the loads behind dy's)
 #pragma unroll
   for (int u = 0; u < KG; ++u) {
     load_code(u, 0);
-    load_idx(u, 1);
+    load_idx(u);
   }
   // the codes of unit u of chunk `of` into the half `h` of A; then its next loads (the index arrived a chunk ago)
   auto stage = [&](int u, int of, int h) {
     *(uint4 *)(sa + (h * UB + u % UB) * ABYTES + wg8_slot<64>(srow, sseg)) = wg8_restore<FMT>(code[u], sc[u]);
     load_code(u, of + 1);
-    load_idx(u, of + 2);
+    load_idx(u);
   };
   constexpr int PH = KG / UB;
   write_dy(0);

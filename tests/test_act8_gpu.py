@@ -376,3 +376,12 @@ def test_a_rewound_arena_is_noticed(act8):
         held.restore()
     with pytest.raises(arena.ArenaError):
         act8.weight_grad(held, rows(4, 8, torch.float32))
+
+
+@pytest.mark.parametrize("n,kvol,cin", [(1, 1, 16), (64, 1, 64), (63, 3, 16), (128, 27, 16), (640, 5, 64), (4096, 27, 32), (8129, 3, 48)])
+def test_tables_that_end_with_their_buffer(act8, n, kvol, cin):
+    """the entries requested ahead of the rows end with the table: the last offset's rows are all there, and nothing behind them counts"""
+    x, dy = rows(n, cin, torch.bfloat16, 1), rows(n, 16, torch.bfloat16, 2)
+    nbr = table(n, n, kvol, 0.5, n)
+    nbr[-1] = torch.arange(n, dtype=torch.int32).flip(0)
+    check_dw(act8.weight_grad(act8.hold(x, "int8"), dy, nbr.cuda()), restored(x, "int8"), dy, nbr)

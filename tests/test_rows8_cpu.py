@@ -112,3 +112,31 @@ def test_python_layer_without_a_gpu():
     for bad in (dict(num_features=0), dict(num_features=8193), dict(num_features=8, kind="group")):
         with pytest.raises(ValueError):
             rownorm.RowNorm(**bad)
+
+
+def test_buffer_loads_carry_their_whole_offset_where_it_is_checked():
+    """The range check of a raw buffer access covers the vector offset; the scalar offset comes on top of it, unchecked.  The weight
+    gradient's table entries are requested up to two chunks of rows ahead and rely on the check behind the table's end, so nothing
+    that moves may stand in the scalar offset: it is the literal 0."""
+    import os
+    import re
+
+    from conftest import ROOT
+
+    place = {"load": 2, "store": 3, "load_lds": 4}  # the scalar offset's place among the arguments
+    seen = 0
+    for name in ("d3d_common.h", "d3d_act8.h", "d3d_act8.hip", "d3d_rownorm.hip"):
+        text = open(os.path.join(ROOT, "det3d_amd", "csrc", name)).read()
+        for m in re.finditer(r"__builtin_amdgcn_raw_(?:ptr_)?buffer_(load_lds|load|store)\w*\(", text):
+            depth, args, at = 1, [""], m.end()
+            while depth:
+                ch = text[at]
+                depth += (ch in "([{") - (ch in ")]}")
+                if ch == "," and depth == 1:
+                    args.append("")
+                elif depth:
+                    args[-1] += ch
+                at += 1
+            seen += 1
+            assert args[place[m.group(1)]].strip() == "0", (name, text[m.start():at])
+    assert seen >= 5

@@ -40,6 +40,12 @@ def pitch(c):
     return (c + GROUP - 1) // GROUP * GROUP
 
 
+def held_bytes(n, c):
+    """size of the buffer that holds n rows of c channels: the codes and one scale a group"""
+    p = pitch(c)
+    return n * (p + p // GROUP)
+
+
 def rows_of(t, what):
     """`t` as the kernels read a matrix of rows: on the GPU, [n, c], float32 or bfloat16, neighbouring channels next to each
     other (any distance between rows; other layouts are copied)"""
@@ -93,8 +99,7 @@ class Held:
 
     @staticmethod
     def room(n, c, dtype, fmt, dev, lease):
-        p = pitch(c)
-        return Held(mem.empty((n * (p + p // GROUP),), torch.uint8, dev, lease.arena), (n, c), dtype, fmt, lease)
+        return Held(mem.empty((held_bytes(n, c),), torch.uint8, dev, lease.arena), (n, c), dtype, fmt, lease)
 
     @property
     def codes(self):

@@ -123,6 +123,11 @@ def _addresses(tensors):
     return [None if t is None else t.data_ptr() for t in tensors]
 
 
+def _strides(x, f, gate):
+    """distances within the rows that a description holds beside their addresses (x, f: rows or 8-bit buffers)"""
+    return x.stride(), None if f is None else f.stride(), None if gate is None else gate.stride()
+
+
 def _gradient(t, dtype, c):
     """(an output's gradient as rows, its address and row stride)"""
     if t is None:
@@ -163,7 +168,7 @@ class _JoinFn(torch.autograd.Function):
             d.h = d.z = None
             if hx is not None:
                 d.x = d.f = None
-        ctx.desc, ctx.at = d, _addresses(saved)
+        ctx.desc, ctx.at, ctx.strides = d, _addresses(saved), _strides(x, f, gate)
         return out
 
     @staticmethod
@@ -197,8 +202,10 @@ class _JoinFn(torch.autograd.Function):
             sums = [next(rows) if need else None for need in (need_s, need_pw, need_pb, need_qw, need_qb)]
         if n:
             d = ctx.desc
-            if _addresses(saved) != ctx.at:  # (saved tensors come back elsewhere: hooks that pack them)
-                d = _elsewhere(call, ctx.lease, saved)
+            # saved tensors that hooks had packed come back elsewhere, and strided ones as a rule contiguous: where the allocator
+            # reuses the address of freed strided rows, the address alone looks like theirs
+            if _addresses(saved) != ctx.at or _strides(*saved[:3]) != ctx.strides:
+                saved, d = _elsewhere(call, ctx.lease, saved)
             ws = mem.empty((ctx.floats,), torch.float32, dev, arena) if ctx.count else None
             g = _lib.RowJoinGrads(dh_at, dh_stride, dz_at, dz_stride, _dp(dx), _dp(df), _dp(dgate), *_addresses(sums), _dp(ws), ctx.floats)
             act8.launch("d3d_row_join_bwd", dev, _lib.lib().d3d_row_join_bwd, ctypes.byref(d), ctypes.byref(g))
@@ -208,14 +215,26 @@ class _JoinFn(torch.autograd.Function):
 
 
 def _elsewhere(call, lease, saved):
-    """the backward pass's description with the saved tensors where they are now"""
-    x, f, gate, scale, post_w, post_b, pre_w, pre_b = saved
+    """(the saved tensors as the kernels read them, the backward pass's description with them where they are now)"""
+    n, c, dtype, dev = call.n, call.c, call.dtype, call.dev
+    rows = ((n, c), dtype) if call.fmt is None else ((act8.held_bytes(n, c),), torch.uint8)
+    vector = ((c,), torch.float32)
+    as_rows = lambda t: act8.rows_of(t, "rownorm")  # noqa: E731
+    plain = as_rows if call.fmt is None else torch.Tensor.contiguous
+    back = []
+    for t, (shape, kind), lay in zip(saved, (rows, rows, ((n, call.gate_cols), dtype)) + (vector,) * 5, (plain, plain, as_rows) + (torch.Tensor.contiguous,) * 5):
+        if t is not None:
+            if tuple(t.shape) != shape or t.dtype != kind or t.device != dev:
+                raise _lib.D3dError("rownorm: a saved tensor came back as %s %s on %s, it was %s %s on %s" % (t.dtype, tuple(t.shape), t.device, kind, shape, dev))
+            t = lay(t)
+        back.append(t)
+    x, f, gate, scale, post_w, post_b, pre_w, pre_b = back
     hx = hf = None
     if call.fmt is not None:
-        hx = act8.Held(x, (call.n, call.c), call.dtype, call.fmt, lease)
-        hf = act8.Held(f, (call.n, call.c), call.dtype, call.fmt, lease) if f is not None else None
+        hx = act8.Held(x, (n, c), dtype, call.fmt, lease)
+        hf = act8.Held(f, (n, c), dtype, call.fmt, lease) if f is not None else None
         x = f = None
-    return call.desc(x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), None, None, hx, hf)
+    return back, call.desc(x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), None, None, hx, hf)
 
 
 def _apply(call, x, f, gate, scale):

@@ -404,3 +404,27 @@ def test_refusals(rn):
     leaf = x.clone().requires_grad_()
     with pytest.raises(D3dError, match="create_graph"):  # no second derivatives, rather than wrong ones
         torch.autograd.grad(rn.norm(leaf, spec).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_strided_rows_that_were_packed_away(rn, checkpoint):
+    """x, f and gate as halves of wider rows that are freed once they are packed: the copies that come back may lie where those lay"""
+    t = make(200, 64, torch.float32, "full")
+    names = ("x", "f", "gate")
+
+    def step(pack):
+        leaf = {k: v.clone().requires_grad_() for k, v in t.items() if k in LEAVES}
+        half = {k: torch.cat([leaf[k], leaf[k]], 1)[:, :64] for k in names}  # rows 128 apart, nobody else's
+        with pack:
+            h, z = rn.join(half["x"], half["f"], post=rn.NormSpec("rms", leaf["post_w"], leaf["post_b"], 1e-5),
+                           pre=rn.NormSpec("layer", leaf["pre_w"], leaf["pre_b"], 1e-5), gate=half["gate"], gate_act="silu",
+                           scale=leaf["scale"], checkpoint=checkpoint)
+        del half
+        return torch.autograd.grad((h, z), list(leaf.values()), (t["dh"], t["dz"]))
+
+    import contextlib
+
+    want = step(contextlib.nullcontext())
+    for _ in range(3):
+        got = step(torch.autograd.graph.save_on_cpu())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -140,3 +140,81 @@ def test_buffer_loads_carry_their_whole_offset_where_it_is_checked():
             seen += 1
             assert args[place[m.group(1)]].strip() == "0", (name, text[m.start():at])
     assert seen >= 5
+
+
+@pytest.fixture
+def launches(hip_lib, monkeypatch):
+    """rownorm on CPU tensors with its launches recorded in place of run: (entry point, copies of its description and gradients)"""
+    from det3d_amd import act8
+
+    seen = []
+
+    def record(what, dev, fn, *args):
+        seen.append((what,) + tuple(type(a._obj).from_buffer_copy(a._obj) for a in args))
+
+    rows_of = lambda t, what: t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()  # noqa: E731
+    monkeypatch.setattr(act8, "launch", record)
+    monkeypatch.setattr(act8, "rows_of", rows_of)
+    return seen
+
+
+def _join_under_hooks(pack, unpack, checkpoint=None):
+    """a join of rows that lie 64 apart, whose saved tensors go through the hooks; (bases, outputs, leaves)"""
+    from det3d_amd import rownorm
+
+    bases = [torch.randn(6, 64) for _ in range(3)]
+    x, f, gate = (b[:, :32].requires_grad_() for b in bases)
+    w = torch.ones(32, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        ends = rownorm.join(x, f, post=rownorm.NormSpec("rms", w, None, 1e-5), pre=rownorm.NormSpec("rms", None, None, 1e-5), gate=gate, checkpoint=checkpoint)
+    return bases, ends, (x, f, gate, w)
+
+
+def _gradients(ends, leaves):
+    return torch.autograd.grad(ends, leaves, (torch.ones(6, 32), torch.ones(6, 32)))
+
+
+def test_saved_rows_that_come_back_with_other_strides_at_their_address(launches):
+    """hooks that pack what is saved give back contiguous copies; where one lies at the address of the strided rows that it was
+    taken from, its rows are read at their new distance"""
+
+    def unpack(t):  # (rows: contiguous, at the strided ones' address)
+        return t if t.dim() == 1 else torch.as_strided(t.detach(), (6, 32), (32, 1))
+
+    bases, ends, leaves = _join_under_hooks(lambda t: t, unpack)
+    _gradients(ends, leaves)
+    (_, fwd), (_, bwd, _) = launches
+    assert (fwd.x_stride, fwd.f_stride, fwd.gate_stride) == (64, 64, 64)
+    assert (bwd.x, bwd.f, bwd.gate) == tuple(b.data_ptr() for b in bases)
+    assert (bwd.x_stride, bwd.f_stride, bwd.gate_stride) == (32, 32, 32)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_saved_tensors_that_come_back_in_another_layout(launches, checkpoint):
+    """columns at a distance, transposed rows, strided vectors and buffers: laid out again before the kernel reads them"""
+    kept = []
+
+    def unpack(t):
+        wide = torch.zeros(t.shape + (2,), dtype=t.dtype)
+        wide[..., 0] = t.detach()
+        kept.append(wide)
+        return wide[..., 0]
+
+    _, ends, leaves = _join_under_hooks(lambda t: t.clone(), unpack, checkpoint)
+    _gradients(ends, leaves)
+    bwd = launches[1][1]
+    strided = {k.data_ptr() for k in kept}
+    rows = (bwd.gate, bwd.post_weight) + ((bwd.x, bwd.f) if checkpoint is None else (bwd.x_codes, bwd.f_codes))
+    assert len(kept) == 4 and not strided & set(rows) and bwd.gate_stride == 32
+    if checkpoint is None:
+        assert (bwd.x_stride, bwd.f_stride) == (32, 32)
+
+
+def test_saved_tensors_that_come_back_as_something_else(launches):
+    from det3d_amd._lib import D3dError
+
+    for unpack in (lambda t: t.bfloat16(), lambda t: t[:1]):
+        _, ends, leaves = _join_under_hooks(lambda t: t.clone(), unpack)
+        with pytest.raises(D3dError, match="came back"):
+            _gradients(ends, leaves)
+    assert all(what == "d3d_row_join_fwd" for what, *_ in launches)

@@ -24,6 +24,7 @@ import ctypes
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _lib, act8, arena as mem, runtime
 
@@ -240,8 +241,13 @@ def _elsewhere(call, lease, saved):
 def _apply(call, x, f, gate, scale):
     _, _, pw, pb = call.post
     _, _, qw, qb = call.pre
+    operands = (x, f, gate, scale, pw, pb, qw, qb)
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (inside a dual level only: asking a tensor takes most of a microsecond)
+        for t in operands:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise _lib.D3dError("rownorm: no forward-mode derivatives (an operand is a dual tensor)")
     if torch.is_grad_enabled():
-        for t in (x, f, gate, scale, pw, pb, qw, qb):
+        for t in operands:
             if t is not None and t.requires_grad:
                 return _JoinFn.apply(call, x, f, gate, scale, pw, pb, qw, qb)
     return _forward(call, x, f, gate, scale, (pw, pb), (qw, qb), None)[0]

@@ -218,3 +218,28 @@ def test_saved_tensors_that_come_back_as_something_else(launches):
         with pytest.raises(D3dError, match="came back"):
             _gradients(ends, leaves)
     assert all(what == "d3d_row_join_fwd" for what, *_ in launches)
+
+
+def test_forward_mode_derivatives_are_refused(launches):
+    """a dual tensor has no requires_grad: without a check its tangent would be dropped, which reads as zero"""
+    from torch.autograd import forward_ad
+
+    from det3d_amd import rownorm
+    from det3d_amd._lib import D3dError
+
+    x, f, w = torch.randn(3, 8), torch.randn(3, 8), torch.ones(8)
+    spec = rownorm.NormSpec("rms", w, None, 1e-5)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        dw = forward_ad.make_dual(w, torch.ones_like(w))
+        for bad in (lambda: rownorm.norm(d, spec), lambda: rownorm.norm(x, spec._replace(weight=dw)), lambda: rownorm.join(x, d, post=spec),
+                    lambda: rownorm.join(x, f, post=spec, gate=d), lambda: rownorm.join(x, f, pre=spec, scale=dw),
+                    lambda: rownorm.norm(d.requires_grad_(), spec)):
+            with pytest.raises(D3dError, match="forward-mode"):
+                bad()
+            with torch.no_grad(), pytest.raises(D3dError, match="forward-mode"):
+                bad()
+        assert not launches
+        rownorm.norm(x, spec)  # plain tensors inside a dual level are nothing special
+    rownorm.norm(x, spec)
+    assert len(launches) == 2

@@ -302,11 +302,13 @@ template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4
     for (int k = 0; k < NV; ++k) {
       const int at = (k * T + lane) * E;
       const bool in = at < c;
+      // (x is read for the pre norm's statistics alone; without it h below is computed from zeros and dropped: a branch around that
+      // too costs the widest f32 rows registers, [4096, 8191] 297 us in place of 274)
       if constexpr (HELD != 0) {
-        rx[k] = in ? Code::fetch(a.x_codes, a.x_scales, row, p.pitch, at) : Code::zero();
+        rx[k] = in && a.pre_kind ? Code::fetch(a.x_codes, a.x_scales, row, p.pitch, at) : Code::zero();
         if (has_f) rf[k] = in ? Code::fetch(a.f_codes, a.f_scales, row, p.pitch, at) : Code::zero();
       } else {
-        rx[k] = in ? Row::template get<ANY>((const char *)a.x + row * a.x_stride * EB, at, c) : Row::zero();
+        rx[k] = in && a.pre_kind ? Row::template get<ANY>((const char *)a.x + row * a.x_stride * EB, at, c) : Row::zero();
         if (has_f) rf[k] = in ? Row::template get<ANY>((const char *)a.f + row * a.f_stride * EB, at, c) : Row::zero();
       }
       rg[k] = in && a.gate_cols > 1 ? Row::template get<ANY>((const char *)a.gate + row * a.gate_stride * EB, at, c) : Row::zero();
@@ -523,13 +525,14 @@ static int rj_check(const D3dRowJoin *a, bool backward, const char *who) {
   D3D_REQUIRE(a->n >= 1 && a->n < ((int64_t)1 << 40) && a->c >= 1 && a->c <= RJ_MAXC, "%s: %lld rows of %d channels (1 to %d)", who,
               (long long)a->n, a->c, RJ_MAXC);
   const bool held = a->x_codes != nullptr;
-  D3D_REQUIRE(a->x || (backward && held), "%s: no rows", who);
+  // (without a pre norm the backward pass does not read x: neither it nor its codes are asked for)
+  D3D_REQUIRE(a->x || (backward && (held || !a->pre_kind)), "%s: no rows", who);
   D3D_REQUIRE(!a->x || a->x_stride >= a->c, "%s: x rows %lld elements apart", who, (long long)a->x_stride);
   D3D_REQUIRE(!a->f || a->f_stride >= a->c, "%s: f rows %lld elements apart", who, (long long)a->f_stride);
   D3D_REQUIRE(held == (a->x_scales != nullptr) && (a->f_codes != nullptr) == (a->f_scales != nullptr), "%s: codes without scales", who);
   const bool has_f = a->f || a->f_codes;
-  D3D_REQUIRE(!has_f || backward || held == (a->f_codes != nullptr), "%s: x and f are held together", who);
   D3D_REQUIRE(!backward || !held || !has_f || a->f_codes, "%s: x is held in 8 bits, f is not", who);
+  D3D_REQUIRE(!has_f || (backward && !a->f_codes) || held == (a->f_codes != nullptr) || (!a->pre_kind && a->f_codes), "%s: x and f are held together", who);
   D3D_REQUIRE(has_f || !a->f_codes, "%s: codes of f without f", who);
   D3D_REQUIRE(a->post_kind >= 0 && a->post_kind <= 2 && a->pre_kind >= 0 && a->pre_kind <= 2, "%s: norm kinds %d, %d", who, a->post_kind, a->pre_kind);
   D3D_REQUIRE(a->post_eps >= 0.f && a->pre_eps >= 0.f, "%s: negative eps", who);
@@ -629,7 +632,7 @@ extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d
   p.inv_c = 1.f / (float)a->c;
   p.pitch = a8_pitch(a->c);
   p.sums = sums;
-  const int held = a->x_codes ? 1 + a->fmt : 0;
+  const int held = (a->pre_kind ? a->x_codes : a->f_codes) ? 1 + a->fmt : 0;
   int blocks = 0;
   rc = rj_for(a, vec, [&](auto shape) {
     using S = decltype(shape);

@@ -12,6 +12,7 @@ None: a factor 1; scale None: alpha alone; pre None: only h comes back.
 
 `checkpoint` ("int8" | "e4m3", act8.py) keeps x and f for the backward pass in 8 bits, written in the same pass as h and z; the
 gradients are then those at the restored rows: exactly what the backward pass of `join(restored x, restored f, ...)` gives.
+x is kept for the pre norm's statistics alone: a join without `pre` keeps f and the gate.
 
 Sums over a row and over the rows (gradients of weights, biases and scales) are float32 in a fixed order: two identical calls
 give the same bits.  Both directions can be captured into a graph; as with any autograd node, an eager graph of the same leaves must
@@ -126,7 +127,7 @@ def _addresses(tensors):
 
 def _strides(x, f, gate):
     """distances within the rows that a description holds beside their addresses (x, f: rows or 8-bit buffers)"""
-    return x.stride(), None if f is None else f.stride(), None if gate is None else gate.stride()
+    return [None if t is None else t.stride() for t in (x, f, gate)]
 
 
 def _gradient(t, dtype, c):
@@ -151,15 +152,18 @@ class _JoinFn(torch.autograd.Function):
     def forward(ctx, call, x, f, gate, scale, post_w, post_b, pre_w, pre_b):
         lease = mem.Lease()
         hx = hf = None
+        keep_x = call.pre[0] != 0  # (dH = dh without a pre norm: the backward pass does not read x)
         if call.fmt is not None:
-            hx = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease)
+            hx = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease) if keep_x else None
             hf = act8.Held.room(call.n, call.c, call.dtype, call.fmt, call.dev, lease) if f is not None else None
         out, d = _forward(call, x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), lease.arena, hx, hf)
         ctx.set_materialize_grads(False)
         ctx.call, ctx.lease = call, lease
         # (in 8 bits the backward pass reads the codes alone: x and f are free once nobody else holds them)
-        if hx is not None:
-            x, f = hx.buf, hf.buf if hf is not None else None
+        if call.fmt is not None:
+            x, f = hx.buf if hx is not None else None, hf.buf if hf is not None else None
+        elif not keep_x:
+            x = None
         saved = (x, f, gate, scale, post_w, post_b, pre_w, pre_b)
         ctx.save_for_backward(*saved)
         _, _, _, _, need_s, need_pw, need_pb, need_qw, need_qb = ctx.needs_input_grad
@@ -167,8 +171,10 @@ class _JoinFn(torch.autograd.Function):
         ctx.floats = _lib.lib().d3d_row_join_ws_floats(call.n, call.c, call.dt, ctx.count) if ctx.count and call.n else 0
         if d is not None:
             d.h = d.z = None
-            if hx is not None:
-                d.x = d.f = None
+            if x is None or hx is not None:
+                d.x = None
+            if hf is not None:
+                d.f = None
         ctx.desc, ctx.at, ctx.strides = d, _addresses(saved), _strides(x, f, gate)
         return out
 
@@ -232,7 +238,7 @@ def _elsewhere(call, lease, saved):
     x, f, gate, scale, post_w, post_b, pre_w, pre_b = back
     hx = hf = None
     if call.fmt is not None:
-        hx = act8.Held(x, (n, c), dtype, call.fmt, lease)
+        hx = act8.Held(x, (n, c), dtype, call.fmt, lease) if x is not None else None
         hf = act8.Held(f, (n, c), dtype, call.fmt, lease) if f is not None else None
         x = f = None
     return back, call.desc(x, f, gate, scale, (post_w, post_b), (pre_w, pre_b), None, None, hx, hf)

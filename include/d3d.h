@@ -500,7 +500,7 @@ int d3d_act8_wgrad(const uint8_t *codes, const uint8_t *scales, int fmt, int64_t
  * contiguous.  f NULL: z = pre(x), h unused.  gate_cols 0 (no gate) | 1 (one value a row) | c.  scale, weights, biases: dev [c]
  * f32 or NULL.  fwd with x_codes / x_scales (and f_codes / f_scales with f) writes x and f in 8 bits of format fmt in the
  * same pass; bwd with them reads the codes in place of x and f (which may then be NULL) and gives the gradients at the restored
- * rows.  z may be NULL without a pre norm.
+ * rows.  Without a pre norm z may be NULL, bwd reads neither x nor its codes (both may be NULL), and fwd takes f_codes alone.
  * bwd: dh, dz dev [n, c] dtype, either NULL = zero; every result may be NULL; dgate [n, gate_cols] dtype; dscale, dpost_*,
  * dpre_* dev [c] f32, overwritten; ws: d3d_row_join_ws_floats(n, c, dtype, number of [c] results asked for) floats. */
 #define D3D_NORM_NONE 0

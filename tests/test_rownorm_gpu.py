@@ -428,3 +428,38 @@ def test_strided_rows_that_were_packed_away(rn, checkpoint):
     for _ in range(3):
         got = step(torch.autograd.graph.save_on_cpu())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("fmt", [None, "int8", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gate,act", [(None, "none"), ("row", "sigmoid"), ("full", "silu")])
+@pytest.mark.parametrize("n,c", [(1, 1), (7, 16), (40, 130), (5, 333), (300, 64), (3, 2500), (2, 8192)])
+def test_a_join_without_a_pre_norm(rn, n, c, gate, act, dtype, fmt):
+    """the residual block's join: its gradients are those at f (held: at the restored f), whatever x was"""
+    from det3d_amd import act8
+
+    t = make(n, c, dtype, gate)
+    at = None if fmt is None else {"f": act8.hold(t["f"], fmt).restore()}
+    _, grads = check(rn, t, "layer" if n % 2 else "rms", None, act, alpha=0.5, checkpoint=fmt, at=at)
+    assert torch.equal(grads["x"], t["dh"])
+    _, other = run(rn, {**t, "x": torch.full_like(t["x"], float("inf"))}, "layer" if n % 2 else "rms", None, act, 0.5, 1e-5, fmt)
+    assert all(torch.equal(grads[k], other[k]) for k in grads)
+
+
+@pytest.mark.parametrize("fmt", [None, "int8"])
+@pytest.mark.parametrize("pre", [False, True])
+def test_what_a_join_keeps(rn, fmt, pre):
+    """bytes between the passes: h (and z), f, and x only where a pre norm's backward pass reads it"""
+    from det3d_amd import act8
+
+    n, c = 40000, 64
+    x, f = rand(n, c, seed=1).requires_grad_(), rand(n, c, seed=2).requires_grad_()
+    spec = rn.NormSpec("rms", None, None, 1e-5)
+    full, held = 4 * n * c, act8.held_bytes(n, c)
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    out = rn.join(x * 1, f * 1, post=spec, pre=spec if pre else None, checkpoint=fmt)
+    kept = torch.cuda.memory_allocated() - base
+    want = full * (2 if pre else 1) + (held if fmt else full) * (2 if pre else 1)
+    assert want <= kept <= want + 4 * (1 << 21), (kept, want)  # (the allocator's blocks: 2 MiB each)
+    del out

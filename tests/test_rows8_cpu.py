@@ -243,3 +243,49 @@ def test_forward_mode_derivatives_are_refused(launches):
         rownorm.norm(x, spec)  # plain tensors inside a dual level are nothing special
     rownorm.norm(x, spec)
     assert len(launches) == 2
+
+
+def test_a_join_without_a_pre_norm_asks_for_no_x(hip_lib):
+    """dH = dh there: the backward pass takes f alone, held or not, and the forward pass writes the codes of f alone"""
+    from det3d_amd import _lib
+
+    L = hip_lib
+
+    def bwd(**kw):  # (the missing workspace is found behind every other check)
+        args = dict(n=100000, c=64, dtype=0, fmt=0, post_kind=1, pre_kind=0, scale=16, f_stride=64)
+        args.update(kw)
+        rc = L.d3d_row_join_bwd(ctypes.byref(_lib.RowJoin(**args)), ctypes.byref(_lib.RowJoinGrads(dh=16, dh_stride=64, dx=16, df=16, dscale=16)), None)
+        return rc, err(L)
+
+    for kw in (dict(f=16), dict(f_codes=16, f_scales=1), dict(f=16, x=16, x_stride=64), dict(f_codes=16, f_scales=1, x_codes=16, x_scales=1)):
+        rc, word = bwd(**kw)
+        assert rc == -2 and b"workspace" in word, (kw, word)
+    for kw, word in ((dict(f=16, pre_kind=1), b"no rows"), (dict(f_codes=16, f_scales=1, pre_kind=1), b"no rows"), (dict(f_codes=16, f_scales=1, x=16, x_stride=64, pre_kind=1), b"together"),
+                     (dict(f=16, x_codes=16, x_scales=1), b"f is not")):
+        rc, got = bwd(**kw)
+        assert rc == -1 and word in got, (kw, got)
+    fwd = lambda **kw: L.d3d_row_join_fwd(ctypes.byref(_lib.RowJoin(**{**dict(n=10, c=64, x=16, x_stride=64, f=16, f_stride=64, pre_kind=0), **kw})), None)  # noqa: E731
+    assert fwd(f_codes=16, f_scales=1) == -1 and b"null output" in err(L)  # (h is what is missing)
+    assert fwd(x_codes=16, x_scales=1) == -1 and b"together" in err(L)
+    assert fwd(f_codes=16, f_scales=1, pre_kind=1) == -1 and b"together" in err(L)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_a_join_without_a_pre_norm_keeps_no_x(launches, checkpoint):
+    """x is neither saved, nor held, nor guarded against a change in place"""
+    from det3d_amd import act8, rownorm
+
+    x, f, gate = (torch.randn(6, 40).requires_grad_() for _ in range(3))
+    w = torch.ones(40, requires_grad=True)
+    stream, kept = x * 1, []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        h = rownorm.join(stream, f, post=rownorm.NormSpec("rms", w, None, 1e-5), gate=gate, checkpoint=checkpoint)
+    sizes = [t.numel() * t.element_size() for t in kept]
+    assert sorted(sizes) == sorted([6 * 40 * 4, 40 * 4, 6 * 40 * 4 if checkpoint is None else act8.held_bytes(6, 40)])
+    with torch.no_grad():
+        stream.add_(1)
+    dx, *_ = torch.autograd.grad(h, (x, f, gate, w), torch.ones(6, 40))
+    assert dx.shape == x.shape
+    (_, fwd), (_, bwd, _) = launches
+    assert fwd.x == stream.data_ptr() and not fwd.x_codes and bool(fwd.f_codes) == (checkpoint is not None)
+    assert not bwd.x and not bwd.x_codes and bool(bwd.f) == (checkpoint is None) and bool(bwd.f_codes) == (checkpoint is not None)

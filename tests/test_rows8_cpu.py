@@ -289,3 +289,11 @@ def test_a_join_without_a_pre_norm_keeps_no_x(launches, checkpoint):
     (_, fwd), (_, bwd, _) = launches
     assert fwd.x == stream.data_ptr() and not fwd.x_codes and bool(fwd.f_codes) == (checkpoint is not None)
     assert not bwd.x and not bwd.x_codes and bool(bwd.f) == (checkpoint is None) and bool(bwd.f_codes) == (checkpoint is not None)
+
+
+def test_codes_of_an_absent_f_are_refused(hip_lib):
+    """a forward pass without f would leave room given for f's codes unwritten"""
+    from det3d_amd import _lib
+
+    a = dict(n=10, c=64, x=16, x_stride=64, pre_kind=1, z=16, x_codes=16, x_scales=1, f_codes=16, f_scales=1)
+    assert hip_lib.d3d_row_join_fwd(ctypes.byref(_lib.RowJoin(**a)), None) == -1 and b"codes of f without f" in err(hip_lib)

@@ -46,6 +46,12 @@ def held_bytes(n, c):
     return n * (p + p // GROUP)
 
 
+def readable(n_in, cin, cout, kvol, cap):
+    """can `weight_grad` read n_in held rows through a table [kvol, cap]?  (It addresses the table and the codes behind it with 32
+    bits: the limits that d3d_act8_wgrad refuses beyond.)"""
+    return n_in < 1 << 24 and n_in * pitch(cin) < (1 << 31) - 16 and kvol * cap < 1 << 29 and kvol <= 4096 and kvol * cin * cout < 1 << 30
+
+
 def rows_of(t, what):
     """`t` as the kernels read a matrix of rows: on the GPU, [n, c], float32 or bfloat16, neighbouring channels next to each
     other (any distance between rows; other layouts are copied)"""
@@ -170,8 +176,9 @@ def weight_grad(held, dy, nbr=None):
         nbr [kvol, cap] int32 (cap >= n_out, as in a Rulebook):  dw[k] = sum_o x[nbr[k][o]]^T dy[o]   -> float32 [kvol, cin, cout]
         nbr None, n_out == n_in (a linear layer, a 1x1 convolution):  dw = x^T dy                     -> float32 [cin, cout]
 
-    Entries of the table outside [0, n_in) are absent neighbours and add nothing.  Products are exact to float32 (bfloat16 `dy`: as
-    they are; float32 `dy`: in three bfloat16 terms), sums are float32 in a fixed order.  A non-finite value in `dy` (float32:
+    Entries of the table outside [0, n_in) are absent neighbours and add nothing.  Behind a table there are limits to the number of
+    held rows and the table's size (`readable`).  Products are exact to float32 (bfloat16 `dy`: as they are; float32 `dy`: in three
+    bfloat16 terms), sums are float32 in a fixed order.  A non-finite value in `dy` (float32:
     also one beyond bfloat16's range, 3.39e38) makes its column of dw non-finite, for every offset: rows meet an absent neighbour as
     a zero."""
     dy = rows_of(dy, "act8.weight_grad")

@@ -493,7 +493,8 @@ class _SparseConvFn(torch.autograd.Function):
         _lib.check(rc, "d3d_sparse_conv_fwd")
         ctx.stats_done = ep is not None
         ctx.feat_dtype, ctx.held = feats.dtype, None
-        if held is not None and ctx.needs_input_grad[1]:  # the weight gradient alone reads the input rows: keep them in 8 bits
+        # the weight gradient alone reads the input rows: keep them in 8 bits (batches beyond its tables' limits in full)
+        if held is not None and ctx.needs_input_grad[1] and act8.readable(rb.n_in, pad_cin, cout, kvol, rb.cap_out):
             rows = act8.hold(feats, held)
             ctx.save_for_backward(rows.buf, weight)
             ctx.held = rows.meta()

@@ -297,3 +297,21 @@ def test_codes_of_an_absent_f_are_refused(hip_lib):
 
     a = dict(n=10, c=64, x=16, x_stride=64, pre_kind=1, z=16, x_codes=16, x_scales=1, f_codes=16, f_scales=1)
     assert hip_lib.d3d_row_join_fwd(ctypes.byref(_lib.RowJoin(**a)), None) == -1 and b"codes of f without f" in err(hip_lib)
+
+
+def test_what_the_weight_gradient_can_read(hip_lib):
+    """act8.readable is what the entry point accepts, on both sides of every limit"""
+    from det3d_amd import act8
+
+    L = hip_lib
+    sides = set()
+    for n_in, cin, cout, kvol, cap in ((1000, 16, 16, 27, 200000), ((1 << 24) - 1, 16, 16, 27, 200000), (1 << 24, 16, 16, 27, 200000), (1 << 22, 511, 16, 1, 200000),
+                                       ((1 << 22) - 1, 512, 16, 1, 200000), (1 << 22, 512, 16, 1, 200000), (1000, 16, 16, 27, (1 << 29) // 27), (1000, 16, 16, 27, (1 << 29) // 27 + 1),
+                                       (1000, 16, 16, 1, 1 << 29), (1000, 1, 1, 4096, 100000), (1000, 1, 1, 4097, 100000)):
+        # (the missing workspace is found behind every other check)
+        rc = L.d3d_act8_wgrad(16, 1, 0, n_in, cin, 1, cout, 0, 100000, cout, 1, cap, kvol, 1, None, 0, None)
+        ok = act8.readable(n_in, cin, cout, kvol, cap)
+        assert rc == (-2 if ok else -1), (n_in, cin, cout, kvol, cap, rc, err(L))
+        sides.add(ok)
+    assert sides == {True, False}
+    assert not act8.readable(10, 1 << 15, 1 << 15, 1, 10) and L.d3d_act8_wgrad(16, 1, 0, 10, 1 << 15, 1, 1 << 15, 0, 10, 1 << 15, 1, 10, 1, 1, None, 0, None) == -1

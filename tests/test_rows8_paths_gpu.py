@@ -277,3 +277,24 @@ def test_a_detector_trains_on_held_rows(mode):
         losses[m] = [float(step(ex)) for _ in range(2)]
     assert abs(losses[mode][0] - losses["full"][0]) <= 1e-4 * abs(losses["full"][0])
     assert all(v == v and abs(v) < 1e6 for v in losses[mode])
+
+
+def test_a_table_beyond_the_8_bit_rows_limits():
+    """a rulebook with room for more entries than the gradient of held rows can address: the layer keeps full rows, and trains"""
+    from det3d_amd import runtime, spconv
+
+    n, kvol, make = 300, 27, sites(n=300, c=16)
+    conv = spconv.SubMConv3d(16, 32, 3, indice_key="a").cuda()
+    with torch.no_grad():
+        rb = conv(make()).indice_dict["a"]
+    cap = (1 << 29) // kvol + 1
+    table = torch.full((kvol, cap), -1, dtype=torch.int32, device="cuda")
+    table[:, :n] = rb.nbr_out.view(kvol, rb.cap_out)[:, :n]
+    got = {}
+    for mode in ("full", "int8"):
+        runtime.configure(activations=mode)
+        x = make()
+        x.indice_dict["a"] = spconv.Rulebook(kvol, cap, cap, table.view(-1), None, None, n, n, x.indices, rb.out_shape, True)
+        y = conv(x).features
+        got[mode] = (y.detach(),) + torch.autograd.grad(y, [x.features, conv.weight, conv.bias], torch.ones_like(y))
+    assert all(torch.equal(a, b) for a, b in zip(got["full"], got["int8"]))

@@ -2,7 +2,8 @@
 
 A layer keeps its input rows for its weight gradient, a normalisation its input for its own backward pass: most of a training
 step's memory.  `hold` keeps such rows `[n, c]` (float32 or bfloat16) as one byte a value: every 32 consecutive channels of a
-row share a scale 2^s (one more byte), so a step holds 1.03 bytes a value in place of 4 or 2.
+row share a scale 2^s (one more byte), so a row of whole groups takes 1.03 bytes a value in place of 4 or 2.  Rows are padded to
+whole groups: one of 16 channels takes 33 bytes, in place of 64 or 32 (`smaller`).
 
     int8   s is the smallest with rint(max|x| 2^-s) <= 127, codes are rint(x 2^-s): off by at most 2^(s-1) = max|x| / 127.5
     e4m3   s is the smallest with max|x| 2^-s <= 448, codes are x 2^-s in e4m3: off by at most 2^-4 of the value, or 2^(s-10)
@@ -44,6 +45,12 @@ def held_bytes(n, c):
     """size of the buffer that holds n rows of c channels: the codes and one scale a group"""
     p = pitch(c)
     return n * (p + p // GROUP)
+
+
+def smaller(c, dtype):
+    """do rows of c channels take less room in 8 bits?  Not where padding to whole groups eats what the codes save: 16 bfloat16
+    channels are 32 bytes a row, held they are 33."""
+    return held_bytes(1, c) < c * dtype.itemsize
 
 
 def readable(n_in, cin, cout, kvol, cap):

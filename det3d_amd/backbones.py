@@ -12,7 +12,7 @@ import numpy as np
 import torch
 from torch import nn
 
-from . import rownorm, runtime, spconv
+from . import rownorm, spconv
 from .nn_utils import build_norm_layer
 from .registry import BACKBONES
 from .rownorm import RowNorm
@@ -82,7 +82,8 @@ class SparseBasicBlock(spconv.SparseModule):
             # a row norm: joined with the identity branch in one pass
             out = self.conv2(out)
             identity = x if self.downsample is None else self.downsample(x)
-            out.features = self.relu(rownorm.join(identity.features, out.features, post=self.bn2, checkpoint=runtime.held_format()))
+            kept = rownorm.kept_format(out.features, self.conv2.out_channels)
+            out.features = self.relu(rownorm.join(identity.features, out.features, post=self.bn2, checkpoint=kept))
             return out
         else:
             out = self.conv2(out)

@@ -282,9 +282,16 @@ def join(x, f, post=None, pre=None, gate=None, gate_act="none", scale=None, alph
     return _apply(call, x, f, gate, _vector(scale, call.c, call.dev, "scale"))
 
 
+def kept_format(x, c):
+    """the `checkpoint` of layers on rows of x's type with c channels, by runtime "activations" ("full" | "int8" | "e4m3"): none where
+    8 bits would not make the rows smaller"""
+    fmt = runtime.held_format()
+    return fmt if fmt is not None and act8.smaller(c, x.dtype) else None
+
+
 class RowNorm(nn.Module):
     """The norm as a module: rows [n, c] (features of a SparseConvTensor), or [b, c, ...] over its channels (pillars, maps).
-    Keeps its input for the backward pass as runtime "activations" says ("full" | "int8" | "e4m3")."""
+    Keeps its input for the backward pass as `kept_format` says."""
 
     def __init__(self, num_features, eps=1e-5, kind="rms", affine=True, bias=None):
         """bias: None = as the kind has it usually (layer: yes, rms: no)"""
@@ -307,7 +314,7 @@ class RowNorm(nn.Module):
 
     def forward(self, x):
         if x.dim() <= 2:
-            return norm(x, self.spec, checkpoint=runtime.held_format())
+            return norm(x, self.spec, checkpoint=kept_format(x, self.num_features))
         y = x.movedim(1, -1)  # (channels-last memory: a view of rows; other maps are copied into that order)
-        z = norm(y.reshape(-1, x.shape[1]), self.spec, checkpoint=runtime.held_format())
+        z = norm(y.reshape(-1, x.shape[1]), self.spec, checkpoint=kept_format(x, self.num_features))
         return z.view(y.shape).movedim(-1, 1)

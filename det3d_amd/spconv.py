@@ -453,6 +453,20 @@ def _kept_format():
     return _runtime.held_format() if torch.is_grad_enabled() else None
 
 
+def _keep(rows, fmt):
+    """(what to save of `rows`, the meta() of what was held or None) for a backward pass at the rows that 8 bits of `fmt` restore.
+    Rows that would be no smaller are saved as they are and held when they are read: what a layer computes is the same."""
+    if fmt is None or not act8.smaller(rows.shape[1], rows.dtype):
+        return rows, None
+    held = act8.hold(rows, fmt)
+    return held.buf, held.meta()
+
+
+def _kept(saved, meta, fmt):
+    """the held rows of _keep's answer"""
+    return act8.Held(saved, *meta) if meta is not None else act8.hold(saved, fmt)
+
+
 class _SparseConvFn(torch.autograd.Function):
     @staticmethod
     @_lib.ctx_forward
@@ -492,14 +506,13 @@ class _SparseConvFn(torch.autograd.Function):
         rc = launch_fwd(rb, feats, wpack, b, pad_cin, cout, out, ep, _lib.stream_ptr(feats.device))
         _lib.check(rc, "d3d_sparse_conv_fwd")
         ctx.stats_done = ep is not None
-        ctx.feat_dtype, ctx.held = feats.dtype, None
+        ctx.feat_dtype = feats.dtype
         # the weight gradient alone reads the input rows: keep them in 8 bits (batches beyond its tables' limits in full)
-        if held is not None and ctx.needs_input_grad[1] and act8.readable(rb.n_in, pad_cin, cout, kvol, rb.cap_out):
-            rows = act8.hold(feats, held)
-            ctx.save_for_backward(rows.buf, weight)
-            ctx.held = rows.meta()
-        else:
-            ctx.save_for_backward(feats, weight)
+        if held is not None and not (ctx.needs_input_grad[1] and act8.readable(rb.n_in, pad_cin, cout, kvol, rb.cap_out)):
+            held = None
+        kept, ctx.held = _keep(feats, held)
+        ctx.fmt = held
+        ctx.save_for_backward(kept, weight)
         ctx.wd = wd
         from . import repack
         ctx.repack_stamp = repack.stamp((weight,))  # `wd` is rewritten in place by Repacker.run()
@@ -548,8 +561,8 @@ class _SparseConvFn(torch.autograd.Function):
                 gin = gin[:, :cin].contiguous()
         if ctx.needs_input_grad[1]:
             gw = torch.empty((kvol, pad_cin, cout), dtype=torch.float32, device=dev)
-            if ctx.held is not None:
-                held = act8.Held(feats, *ctx.held)
+            if ctx.fmt is not None:
+                held = _kept(feats, ctx.held, ctx.fmt)
                 _timed("wgrad", pad_cin, cout, rb.n_out, rb, dev, lambda: act8.launch_weight_grad(
                     held, gout, rb.nbr_out.data_ptr(), rb.cap_out, kvol, gw))
             else:
@@ -593,13 +606,9 @@ class _BNReLUFn(torch.autograd.Function):
                             save[0].data_ptr(), save[1].data_ptr(), st)
         _lib.check(rc, "d3d_bn_apply")
         # in 8 bits the backward sweeps read the restored rows (with the statistics of the full ones)
-        ctx.held = None
-        if held is not None and training and link is None and any(ctx.needs_input_grad[:3]):
-            rows = act8.hold(x, held)
-            ctx.save_for_backward(rows.buf, weight, bias, save)
-            ctx.held = rows.meta()
-        else:
-            ctx.save_for_backward(x, weight, bias, save)
+        ctx.fmt = held if training and link is None and any(ctx.needs_input_grad[:3]) else None
+        kept, ctx.held = _keep(x, ctx.fmt)
+        ctx.save_for_backward(kept, weight, bias, save)
         ctx.relu = relu
         ctx.training = training
         ctx.link = link
@@ -618,8 +627,8 @@ class _BNReLUFn(torch.autograd.Function):
             raise _lib.D3dError("fused sparse BN backward is implemented for training mode only")
         L = _lib.lib()
         x, weight, bias, save = ctx.saved_tensors
-        if ctx.held is not None:
-            x = act8.Held(x, *ctx.held).restore()
+        if ctx.fmt is not None:
+            x = _kept(x, ctx.held, ctx.fmt).restore()
         n, c = x.shape
         dy = dy.contiguous().to(x.dtype)
         A = ctx.lease.check("sparse BatchNorm")

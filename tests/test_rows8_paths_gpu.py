@@ -298,3 +298,38 @@ def test_a_table_beyond_the_8_bit_rows_limits():
         y = conv(x).features
         got[mode] = (y.detach(),) + torch.autograd.grad(y, [x.features, conv.weight, conv.bias], torch.ones_like(y))
     assert all(torch.equal(a, b) for a, b in zip(got["full"], got["int8"]))
+
+
+def test_rows_that_8_bits_do_not_make_smaller(monkeypatch):
+    """16 bfloat16 channels are 32 bytes a row, held they are 33: such rows are kept as they are, with the gradients of held ones"""
+    from det3d_amd import act8, runtime, spconv
+    from det3d_amd.rownorm import RowNorm
+
+    assert not act8.smaller(16, torch.bfloat16) and act8.smaller(24, torch.bfloat16) and act8.smaller(16, torch.float32)
+    n, c = 1500, 16
+    make = sites(n=n, c=c, dtype=torch.bfloat16)
+    torch.manual_seed(0)
+    conv = spconv.SubMConv3d(c, 32, 3, indice_key="a").cuda()
+    bn = nn.BatchNorm1d(c, eps=1e-3, momentum=0.01).cuda().train()
+    norm = RowNorm(c).cuda()
+    runtime.configure(activations="int8")
+
+    def step():
+        kept, rows = [], make()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.numel() * t.element_size()) or t, lambda t: t):
+            rows.features = spconv.bn_relu(bn, rows.features, True)
+            y = conv(rows).features
+        params = [conv.weight, bn.weight, bn.bias]
+        return [k for k in kept if k % n == 0], torch.autograd.grad(y, params, torch.ones_like(y))
+
+    kept, got = step()
+    assert kept == [32 * n] * 2  # (what the sweep and the layer read)
+    monkeypatch.setattr(act8, "smaller", lambda *a: True)
+    kept, want = step()
+    assert kept == [33 * n] * 2
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    monkeypatch.undo()
+    x, kept = make().features, []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.numel() * t.element_size()) or t, lambda t: t):
+        norm(x)
+    assert max(kept) == 32 * n

@@ -603,10 +603,19 @@ extern "C" int d3d_row_join_fwd(const D3dRowJoin *a, d3d_stream_t stream_) {
   return D3D_OK;
 }
 
-// workspace of the column sums: an upper bound over the row layouts (rows per block), which depend on alignment too
+// workspace of the column sums: the blocks' slabs, of one pair of sums where a single result is asked for (two results may belong to
+// different pairs).  The rows of a block follow from the width and the type alone
 extern "C" size_t d3d_row_join_ws_floats(int64_t n, int c, int dtype, int sums) {
   if (n < 1 || c < 1 || c > RJ_MAXC || sums < 1 || sums > 5 || (dtype != D3D_F32 && dtype != D3D_BF16)) return 0;
-  return (size_t)rj_blocks_bwd(n, 1, 256) * 4 * (size_t)c;
+  D3dRowJoin a;
+  memset(&a, 0, sizeof(a));
+  a.c = c;
+  a.dtype = dtype;
+  const int blocks = rj_for(&a, true, [&](auto shape) {
+    using S = decltype(shape);
+    return rj_blocks_bwd(n, S::RPB, S::NT);
+  });
+  return (size_t)blocks * rj_slabs(sums == 1 ? 1 : 3) * (size_t)c;
 }
 
 extern "C" int d3d_row_join_bwd(const D3dRowJoin *a, const D3dRowJoinGrads *g, d3d_stream_t stream_) {

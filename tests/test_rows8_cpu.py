@@ -315,3 +315,20 @@ def test_what_the_weight_gradient_can_read(hip_lib):
         sides.add(ok)
     assert sides == {True, False}
     assert not act8.readable(10, 1 << 15, 1 << 15, 1, 10) and L.d3d_act8_wgrad(16, 1, 0, 10, 1 << 15, 1, 1 << 15, 0, 10, 1 << 15, 1, 10, 1, 1, None, 0, None) == -1
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,c", [(1, 1), (100, 64), (5000, 24), (2057, 333), (100000, 64), (8192, 4096), (3000, 8192), (1 << 33, 16)])
+def test_the_workspace_of_the_column_sums_is_what_they_need(hip_lib, n, c, dtype):
+    """one float less is refused: for all five results, and for one alone"""
+    from det3d_amd import _lib
+
+    L = hip_lib
+    for count, names in ((5, ("dscale", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias")), (1, ("dpre_weight",)), (1, ("dpost_bias",))):
+        need = L.d3d_row_join_ws_floats(n, c, dtype, count)
+        a = _lib.RowJoin(n=n, c=c, dtype=dtype, x=16, x_stride=c, f=16, f_stride=c, scale=16, pre_kind=1, post_kind=1, post_weight=16, post_bias=16, pre_weight=16, pre_bias=16)
+        g = _lib.RowJoinGrads(dh=16, dh_stride=c, dz=16, dz_stride=c, ws=16, ws_floats=need - 1, **{k: 16 for k in names})
+        assert need > 0 and need % c == 0
+        assert L.d3d_row_join_bwd(ctypes.byref(a), ctypes.byref(g), None) == -2 and b"workspace" in err(L), (count, need)
+    if (n, c, dtype) == (8192, 4096, 1):
+        assert L.d3d_row_join_ws_floats(n, c, dtype, 5) * 4 == 512 * 4 * 4096 * 4  # 34 MB: two blocks of 512 threads a CU

@@ -157,7 +157,11 @@ class Held:
             if tuple(out.shape) != (n, c) or out.device != dev or (c > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < c):
                 raise _lib.D3dError("act8.restore: out must be [%d, %d] on %s with neighbouring channels next to each other and "
                                     "rows that do not overlap" % (n, c, dev))
+            if out.requires_grad and torch.is_grad_enabled():
+                raise _lib.D3dError("act8.restore: out requires a gradient, which what is written does not carry")
             stride = row_stride(out)
+            if not out.is_inference():  # (a graph that saved `out` is to notice)
+                torch.autograd.graph.increment_version(out)
         if n:
             codes, scales = self.pointers()
             launch("d3d_act8_restore", dev, _lib.lib().d3d_act8_restore, codes, scales, n, c, FORMATS[self.fmt], _DT[out.dtype],

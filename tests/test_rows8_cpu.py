@@ -150,7 +150,7 @@ def launches(hip_lib, monkeypatch):
     seen = []
 
     def record(what, dev, fn, *args):
-        seen.append((what,) + tuple(type(a._obj).from_buffer_copy(a._obj) for a in args))
+        seen.append((what,) + tuple(type(a._obj).from_buffer_copy(a._obj) for a in args if hasattr(a, "_obj")))
 
     rows_of = lambda t, what: t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()  # noqa: E731
     monkeypatch.setattr(act8, "launch", record)
@@ -332,3 +332,22 @@ def test_the_workspace_of_the_column_sums_is_what_they_need(hip_lib, n, c, dtype
         assert L.d3d_row_join_bwd(ctypes.byref(a), ctypes.byref(g), None) == -2 and b"workspace" in err(L), (count, need)
     if (n, c, dtype) == (8192, 4096, 1):
         assert L.d3d_row_join_ws_floats(n, c, dtype, 5) * 4 == 512 * 4 * 4096 * 4  # 34 MB: two blocks of 512 threads a CU
+
+
+def test_restoring_into_a_tensor_is_a_change_in_place(launches):
+    """as with any operation in place: a graph that saved `out` notices, a leaf that wants a gradient is refused"""
+    from det3d_amd import act8
+    from det3d_amd._lib import D3dError
+
+    held, out, w = act8.hold(torch.randn(4, 32)), torch.ones(4, 32), torch.ones(4, 32, requires_grad=True)
+    y = out * w
+    assert held.restore(out=out) is out
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(D3dError, match="requires a gradient"):
+        held.restore(out=w)
+    with torch.no_grad():
+        held.restore(out=w)
+    with torch.inference_mode():
+        held.restore(out=torch.empty(4, 32))
+    assert [what for what, *_ in launches] == ["d3d_act8_hold"] + 3 * ["d3d_act8_restore"]

@@ -58,7 +58,10 @@ template <bool BF16_, int T_, int NV_, bool ANY_> struct RjShape {
   static constexpr int NT = T > 256 ? T : 256, RPB = NT / T, EPL = E * NV;
 };
 
-// act(g) and, with DA, its derivative.  exp and reciprocal are the hardware's (one step off at most): 1 / (1 + 2^(-g log2 e))
+// act(g) and, with DA, its derivative: p = 1 / (1 + 2^(-g log2 e)).  Exponential and reciprocal are the hardware's, one step off at
+// most each; what is rounded in the exponent weighs |g|, so p is off by at most (1.25 |g| + 5) 2^-24 of its value (sigmoid(-10) by 9
+// steps), and below the smallest normal number (g < -87.3) by as much as that.  The slope is p - p p: for large g, where it
+// vanishes, off by at most 5 2^-24 in all
 template <bool DA> __device__ __forceinline__ void rj_act(int act, float g, float &a, float &da) {
   const float p = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f));
   if (act == D3D_GATE_SIGMOID) {

@@ -463,3 +463,32 @@ def test_what_a_join_keeps(rn, fmt, pre):
     want = full * (2 if pre else 1) + (held if fmt else full) * (2 if pre else 1)
     assert want <= kept <= want + 4 * (1 << 21), (kept, want)  # (the allocator's blocks: 2 MiB each)
     del out
+
+
+def test_activations_far_from_zero(rn):
+    """sigmoid, SiLU and their slopes by relative error.  With u = 2^-24: the exponent -g log2 e is rounded twice (1.25 u of it, with the
+    constant's own error), which is 1.25 |g| u of the exponential; that and the reciprocal are a step (2 u) off, the sum u: p by
+    (1.25 |g| + 5) u.  SiLU adds a product.  Slopes: p - p p, off by p's error and 2 u where p is small, 5 u in all where it is near 1"""
+    g = torch.cat([torch.linspace(-85, 85, 4097), torch.tensor([-80.0, -50.0, -20.0, -10.0, -1e-3, 0.0, 1e-30, 20.0])]).cuda()
+    n = g.numel()
+    one, zero = torch.ones(n, 1, device="cuda"), torch.zeros(n, 1, device="cuda")
+    # (two channels with the same gate: a full gate, h = act(g) exactly)
+    f, x = one.expand(n, 2).contiguous(), zero.expand(n, 2).contiguous()
+    g64 = g.cpu().double()
+    p = 1 / (1 + torch.exp(-g64))
+    rel = (1.25 * g64.abs() + 5) * EPS32
+    for act, want, slope in (("sigmoid", p, p * (1 / (1 + torch.exp(g64)))), ("silu", g64 * p, p * (1 + g64 / (1 + torch.exp(g64))))):
+        gate = g[:, None].expand(n, 2).contiguous().requires_grad_()
+        h = rn.join(x, f, gate=gate, gate_act=act)
+        off = (h.detach()[:, 1].cpu().double() - want).abs()
+        assert (off <= (rel + (act == "silu") * EPS32) * want.abs()).all(), (act, float((off / want.abs().clamp(min=1e-300) / EPS32).max()))
+        (dg,) = torch.autograd.grad(h, gate, torch.ones_like(h))
+        off = (dg[:, 0].cpu().double() - slope).abs()
+        if act == "sigmoid":
+            tol = (rel + 2 * EPS32) * slope + 5 * EPS32 * (g64 > 0)
+        else:  # p + a (1 - p): both terms by p's error, the second with |g|'s weight, three roundings
+            tol = (rel + 3 * EPS32) * (p + g64.abs() * p / (1 + torch.exp(g64))) + 5 * EPS32 * g64.abs() * p * (g64 > 0)
+        assert (off <= tol).all(), (act, float(((off - tol) / EPS32).max()))
+    far = torch.tensor([[-1e30, -1e30], [-100.0, -88.0], [100.0, 1e30], [float("inf"), float("-inf")]], device="cuda")
+    h = rn.join(torch.zeros_like(far), torch.ones_like(far), gate=far, gate_act="sigmoid").cpu()
+    assert (h[:2] <= 2.0 ** -126).all() and (h[:2] >= 0).all() and (h[2] == 1).all() and h[3].tolist() == [1.0, 0.0]

@@ -333,3 +333,92 @@ def test_rows_that_8_bits_do_not_make_smaller(monkeypatch):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.numel() * t.element_size()) or t, lambda t: t):
         norm(x)
     assert max(kept) == 32 * n
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("kind", ["RMS", "LN"])
+def test_a_residual_block_with_row_norms_on_held_rows(kind, fmt):
+    """the values are those of full rows; every gradient is the formula's at what 8 bits restore of the rows that its layer kept,
+    with the ReLUs' signs of the forward pass.  The reference takes the convolutions in full precision mode (split products, 2^-16;
+    a dozen of them behind each other, sums no more than ten times their norm: 1e-3) and the norms as float64 formulas"""
+    from det3d_amd import act8, rownorm, runtime
+    from det3d_amd.backbones import SparseBasicBlock
+
+    torch.manual_seed(0)
+    block = SparseBasicBlock(32, 32, norm_cfg=dict(type=kind, eps=1e-3), indice_key="r").cuda().train()
+    with torch.no_grad():
+        for m in (block.bn1, block.bn2):
+            m.weight.uniform_(0.5, 1.5)
+    make, params = sites(c=32), list(block.parameters())
+    full = block(make()).features.detach()
+    runtime.configure(activations=fmt)
+    x = make()
+    y = block(x).features
+    assert torch.equal(y.detach(), full)
+    dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(5)).cuda()
+    got = torch.autograd.grad(y, [x.features] + params, dy)
+    runtime.configure(activations="full")
+
+    def at(v, r):  # the value v with the gradient of r
+        return v.detach() + (r - r.detach())
+
+    def restored(v):
+        return at(act8.hold(v.detach(), fmt).restore(), v)
+
+    def formula(m, v):
+        v = v.double()
+        if kind == "LN":
+            v = v - v.mean(1, keepdim=True)
+        v = v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-3) * m.weight.double()
+        return (v + m.bias.double() if m.bias is not None else v).float()
+
+    def conv(layer, tensor, feats):
+        """the layer's output, its data gradient, and the weight gradient at the restored rows"""
+        import copy
+
+        still = copy.deepcopy(layer).requires_grad_(False)
+        value = tensor.__class__(feats, tensor.indices, tensor.spatial_shape, tensor.batch_size)
+        value.indice_dict = tensor.indice_dict
+        rows = tensor.__class__(restored(feats).detach(), tensor.indices, tensor.spatial_shape, tensor.batch_size)
+        rows.indice_dict = tensor.indice_dict
+        r = layer(rows).features
+        return still(value).features + (r - r.detach())
+
+    x = make()
+    block(x)  # (the rulebook)
+    f1 = conv(block.conv1, x, x.features)
+    with torch.no_grad():
+        n1 = rownorm.norm(f1, block.bn1)
+    a = torch.relu(at(n1, formula(block.bn1, restored(f1))))
+    f2 = conv(block.conv2, x, a)
+    with torch.no_grad():
+        h = rownorm.join(x.features, f2, post=block.bn2)
+    want_y = torch.relu(at(h, x.features + formula(block.bn2, restored(f2))))
+    assert torch.equal(want_y.detach(), full)
+    want = torch.autograd.grad(want_y, [x.features] + params, dy)
+    for name, g, w in zip(["x"] + [k for k, _ in block.named_parameters()], got, want):
+        assert float((g - w).norm()) <= 1e-3 * float(w.norm()), name
+
+
+@pytest.mark.parametrize("mode,per_value", [("full", 4 + 4 + 4 + 4), ("int8", 3 * 33 / 32 + 4 + 4)])
+def test_what_a_residual_block_with_row_norms_keeps(mode, per_value):
+    """bytes a value between the passes.  Full: what the first norm and the join read, the first ReLU's output (the second
+    convolution's rows too), the second's.  In 8 bits: the rows of the second convolution, the norm and the join, and both ReLUs'
+    outputs, which torch keeps as they are; the first convolution's rows belong to the block before"""
+    from det3d_amd import act8, runtime
+    from det3d_amd.backbones import SparseBasicBlock
+
+    n, c = 60000, 64
+    block = SparseBasicBlock(c, c, norm_cfg=dict(type="RMS", eps=1e-3), indice_key="r").cuda().train()
+    make = sites(n=n, shape=(30, 60, 60), c=c)
+    x = make()
+    with torch.no_grad():
+        block(x)
+    runtime.configure(activations=mode)
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    y = block(x).features
+    kept = torch.cuda.memory_allocated() - base
+    kept -= act8.held_bytes(n, c) if mode == "int8" else 0
+    assert abs(kept / (n * c) - per_value) < 0.05 * per_value, kept / (n * c)
+    del y

@@ -492,3 +492,34 @@ def test_activations_far_from_zero(rn):
     far = torch.tensor([[-1e30, -1e30], [-100.0, -88.0], [100.0, 1e30], [float("inf"), float("-inf")]], device="cuda")
     h = rn.join(torch.zeros_like(far), torch.ones_like(far), gate=far, gate_act="sigmoid").cpu()
     assert (h[:2] <= 2.0 ** -126).all() and (h[:2] >= 0).all() and (h[2] == 1).all() and h[3].tolist() == [1.0, 0.0]
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("pre", [None, "layer"])
+def test_one_tensor_in_every_place_and_two_backward_passes(rn, pre, checkpoint):
+    """x, f and gate are the same rows, the output's gradient is expanded from one number, the graph is gone through twice"""
+    from det3d_amd import act8
+
+    n, c = 50, 64
+    v, w = rand(n, c, seed=3), 1 + rand(c, seed=4, scale=0.3)
+    leaf, weight = v.clone().requires_grad_(), w.clone().requires_grad_()
+    post, pre_s = rn.NormSpec("rms", weight, None, 1e-5), rn.NormSpec(pre, weight, None, 1e-5) if pre else None
+    out = rn.join(leaf, leaf, post=post, pre=pre_s, gate=leaf, gate_act="sigmoid", checkpoint=checkpoint)
+    total = out[0].sum() + 2 * out[1].sum() if pre else out.sum()
+    first = torch.autograd.grad(total, [leaf, weight], retain_graph=True)
+    second = torch.autograd.grad(total, [leaf, weight])
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    # the definition: x and f at the rows that the checkpoint restores, the gate as it came
+    at = act8.hold(v, checkpoint).restore() if checkpoint else v
+    one = torch.ones(n, c, device="cuda")
+    t = {"x": at, "f": at, "gate": v, "scale": None, "post_w": w, "post_b": None, "pre_w": w if pre else None, "pre_b": None, "dh": one, "dz": 2 * one}
+    d64 = {k: a.cpu().double() if a is not None else None for k, a in t.items()}
+    l64 = {k: a.clone().requires_grad_() if k in LEAVES and a is not None else a for k, a in d64.items()}
+    ends = forward64(l64, "rms", pre, "sigmoid", 1.0, 1e-5)
+    names = [k for k in LEAVES if l64.get(k) is not None]
+    want = dict(zip(names, torch.autograd.grad(sum((e * d64["d" + k]).sum() for k, e in ends.items()), [l64[k] for k in names])))
+    M = magnitudes(d64, "rms", pre, "sigmoid", 1.0, 1e-5)
+    for got, parts, k in ((first[0], ("x", "f", "gate"), 512 + 3), (first[1], ("post_w", "pre_w") if pre else ("post_w",), 512 + 4 * n + 2)):
+        off = (got.cpu().double() - sum(want[p] for p in parts)).abs()
+        tol = k * EPS32 * sum(M[p] for p in parts)
+        assert (off <= tol).all(), float((off - tol).max())

@@ -422,3 +422,35 @@ def test_what_a_residual_block_with_row_norms_keeps(mode, per_value):
     kept -= act8.held_bytes(n, c) if mode == "int8" else 0
     assert abs(kept / (n * c) - per_value) < 0.05 * per_value, kept / (n * c)
     del y
+
+
+@pytest.mark.parametrize("mode", ["full", "int8", "e4m3"])
+@pytest.mark.parametrize("shape", [(2, 24, 9, 7), (5, 40, 11)])
+def test_gradients_of_row_norms_on_maps(shape, mode):
+    """maps in either memory order: the gradients of float64 formulas, under 8 bits those at the restored rows"""
+    from det3d_amd import act8, runtime
+    from det3d_amd.rownorm import RowNorm
+
+    c = shape[1]
+    torch.manual_seed(0)
+    m = RowNorm(c, kind="layer").cuda()
+    with torch.no_grad():
+        m.weight.uniform_(0.5, 1.5)
+    runtime.configure(activations=mode)
+    v, g = torch.randn(shape, device="cuda"), torch.randn(shape, device="cuda")
+    for lay in (lambda t: t, lambda t: t.movedim(1, -1).contiguous().movedim(-1, 1)):
+        x = lay(v).clone(memory_format=torch.preserve_format).requires_grad_()
+        dx, dw, db = torch.autograd.grad(m(x), [x, m.weight, m.bias], g)
+        rows, dz = v.movedim(1, -1).reshape(-1, c), g.movedim(1, -1).reshape(-1, c).double()
+        at = (rows if mode == "full" else act8.hold(rows, mode).restore()).double()
+        hat = at - at.mean(1, keepdim=True)
+        r = 1 / torch.sqrt((hat * hat).mean(1, keepdim=True) + 1e-5)
+        hat = hat * r
+        d = dz * m.weight.detach().double()
+        want = r * (d - d.mean(1, keepdim=True) - hat * (d * hat).mean(1, keepdim=True))
+        # (three sums of at most c terms, a dozen roundings, rows of deviation 1 and |hat| <= sqrt(c): 512 steps of the terms' sum)
+        mag = r * (d.abs() + d.abs().mean(1, keepdim=True) + (hat.abs() + r) * (d * hat).abs().mean(1, keepdim=True))
+        assert ((dx.movedim(1, -1).reshape(-1, c).double() - want).abs() <= 512 * 2.0 ** -24 * mag).all()
+        n = rows.shape[0]
+        assert ((dw.double() - (dz * hat).sum(0)).abs() <= (512 + 4 * n) * 2.0 ** -24 * (dz.abs() * (hat.abs() + r)).sum(0)).all()
+        assert ((db.double() - dz.sum(0)).abs() <= (512 + 4 * n) * 2.0 ** -24 * dz.abs().sum(0)).all()

@@ -187,11 +187,11 @@ def weight_grad(held, dy, nbr=None):
         nbr [kvol, cap] int32 (cap >= n_out, as in a Rulebook):  dw[k] = sum_o x[nbr[k][o]]^T dy[o]   -> float32 [kvol, cin, cout]
         nbr None, n_out == n_in (a linear layer, a 1x1 convolution):  dw = x^T dy                     -> float32 [cin, cout]
 
-    Entries of the table outside [0, n_in) are absent neighbours and add nothing.  Behind a table there are limits to the number of
-    held rows and the table's size (`readable`).  Products are exact to float32 (bfloat16 `dy`: as they are; float32 `dy`: in three
-    bfloat16 terms), sums are float32 in a fixed order.  A non-finite value in `dy` (float32:
-    also one beyond bfloat16's range, 3.39e38) makes its column of dw non-finite, for every offset: rows meet an absent neighbour as
-    a zero."""
+    Takes values only, as `hold` does.  Entries of the table outside [0, n_in) are absent neighbours and add nothing; behind a table
+    there are limits to the held rows and the table's size (`readable`).  Products are exact to float32 (bfloat16 `dy`: as they are;
+    float32 `dy`: in three bfloat16 terms, exact from 2^-110 on, smaller values off by at most 2^-134), sums are float32 in a fixed
+    order.  A non-finite value in `dy` (float32: also one beyond bfloat16's range, 3.39e38) makes its column of dw non-finite, for
+    every offset: rows meet an absent neighbour as a zero."""
     dy = rows_of(dy, "act8.weight_grad")
     n_in, cin = held.shape
     n_out, cout = dy.shape

@@ -106,8 +106,9 @@ extern "C" int d3d_act8_restore(const uint8_t *codes, const uint8_t *scales, int
 //
 // A matrix product whose long axis, the rows o, is the outer one of both operands.  Bound by the matrix pipe and by the vector work
 // that restores the codes and splits dy, which overlap in part (without the one or the other 46 to 50 us of 57).  65021 sites, 27
-// offsets, 64 -> 64 channels, f32: 54 us, 800 TFLOP/s of bf16 products with the absent neighbours' zeros; [16384, 1024] x
-// [16384, 1024] bf16: 45 us, 760 TFLOP/s, and 11 us to fold the row ranges; 80003 sites, 16 -> 16 bf16: 20 us, bound by the gathers.
+// offsets, 64 -> 64 channels, f32: 54 us, 800 TFLOP/s of bf16 products with the absent neighbours' zeros (every second entry);
+// [16384, 1024] x [16384, 1024] bf16: 44 us, 780 TFLOP/s, and 11 us to fold the row ranges; 80003 sites, 16 -> 16 bf16: 20 us, bound by
+// the gathers: a CU is busy for 38 thousand cycles, the cache is accessed in 21 of them, vector work issues in 9, the waves wait in half.
 //
 // The (k, ci) axis is flattened (ci padded to 8) and cut into units of 64 columns, so narrow layers fill a unit with several
 // offsets.  A block of 8 waves owns KG units x TN columns of dy and a range of rows, 64 rows (a chunk) at a time:
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(512, 2) a8_wgrad_kernel(Wg8Args p) {
   d3d_lds_barrier();
   // A phase multiplies UB units and meanwhile stages the next UB (behind the chunk's last: the next chunk's first, and its dy).
   // Written with the vector work between the MFMAs, which leave its pipe free: done one after the other, MFMA, restoring and
-  // LDS add up (43 + 47 + 26 thousand cycles of 121 at 64 -> 64 channels, f32).
+  // LDS add up (43 + 47 + 27 thousand cycles at 64 -> 64 channels, f32, where a CU is now busy for 100).
   for (int chunk = 0; chunk < chunks; ++chunk) {
     a8_bf16x8 bf[KS][NB][P];
     const unsigned char *const dcur = sd + (chunk & 1) * P * DBYTES;

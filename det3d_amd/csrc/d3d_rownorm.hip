@@ -11,9 +11,10 @@
 // first gave: no cancellation.  The backward pass recomputes u, h and their statistics from x and f (or from their 8-bit
 // codes) instead of reading saved ones.
 //
-// Join of [8192, 4096] bf16 with both norms, a full gate and e4m3 rows: forward 78 us (404 MB, 5.2 TB/s), backward 137 us (471 MB,
-// 3.4 TB/s: about 750 vector instructions a row and wave, the issue of the SIMDs is two thirds of it), fold 8 us.  Norm of
-// [60013, 128] f32 with int8 rows: forward 17 us, backward 15 us (70 MB each), fold 5 us.
+// Join of [8192, 4096] bf16 with both norms, a full gate and e4m3 rows: forward 76 us (404 MB, 5.3 TB/s), backward 137 us (471 MB,
+// 3.4 TB/s: 700 vector instructions a row and wave, which the SIMDs issue in two thirds of the time), fold 8 us.  Norm of
+// [60013, 128] f32 with int8 rows: forward 15 to 20 us, backward 15 us (70 MB each), fold 5 us.  Join of [65021, 64] f32 with the post
+// norm alone: forward 10.5 us (50 MB), backward 14 (67 MB), with f in int8 12.6 and 12.6 (54 MB each), fold 5.
 #include "d3d_act8.h"
 #include <string.h>
 #include <type_traits>
@@ -260,10 +261,10 @@ template <class S> __device__ __forceinline__ void rj_shared(const float *w, int
   for (int j = 0; j < S::E; j += 4) *(float4 *)(v + j) = *(const float4 *)(w + at + j);
 }
 
-// The backward pass keeps x, f, act and dH of a row in registers, five column sums over the rows beside them (40 registers of a
-// lane with 8 values), and the [c] vectors in LDS: with those in registers too it takes 180 of them, two waves to a SIMD in
-// place of four, and [8192, 4096] bf16 took 201 us in
-// place of 169 (137 now: no lane branches around its part of the vectors, and the sums over lanes leave LDS alone).
+// The backward pass keeps x (then h), f, dH and the gate of a row in registers, four column sums over the rows beside them (32
+// registers of a lane with 8 values), and the [c] vectors in LDS: with those in registers too it takes 180 of them, two waves to a
+// SIMD in place of four, and [8192, 4096] bf16 took 201 us in place of 169 (137 now: no lane branches around its part of the
+// vectors, and the sums over lanes leave LDS alone).
 // HELD: 0 rows as they are, 1 + format: codes
 template <class S, int HELD> __global__ void __launch_bounds__(S::NT, S::EPL > 4 && S::NT < 512 ? 3 : 4) row_join_bwd_kernel(RjArgs p) {
   constexpr int E = S::E, T = S::T, NV = S::NV, EB = S::BF16 ? 2 : 4;
@@ -561,8 +562,8 @@ static bool rj_vectors(const D3dRowJoin *a, const D3dRowJoinGrads *g) {
   return v;
 }
 
-// The shape of the launch by the number of 16-byte vectors in a row: the fewest lanes that hold it with at most 8 values a lane.
-// go(RjShape) launches.
+// The shape of the launch by the number of 16-byte vectors in a row: the fewest lanes that hold it with one vector each (4 values in
+// f32, 8 in bf16); f32 rows of more than 512 vectors take two a lane.  go(RjShape) launches.
 template <bool BF16, bool ANY, class Go> static int rj_pick(int c, Go &&go) {
   const int units = (c + (BF16 ? 8 : 4) - 1) / (BF16 ? 8 : 4);
   if (units <= 8) return go(RjShape<BF16, 8, 1, ANY>{});

@@ -22,10 +22,11 @@ runs keep working), but the authoritative state is here and is settable from cod
                    f32 alike, profiles/round6_stack_executor.txt) -- it is not the interpreter that bounds the host
                    [D3D_STACK_EXECUTOR]
   activations      "full" | "int8" | "e4m3": what the sparse convolutions, the BatchNorm sweeps behind them and RowNorm keep for the
-                   backward pass -- their rows as they are, or in 8 bits (act8.py) where those are smaller.  The one switch here that changes what a
-                   step computes: gradients are taken at the restored rows.  In 8 bits the layers run one by one (the fused
-                   sparse nodes keep full rows) and TrainStep leaves its step arena aside, so that rows are freed as the
-                   forward pass goes on; default "full"                                               [D3D_ACTIVATIONS]
+                   backward pass -- their rows as they are, or in 8 bits (act8.py) where those are smaller.  The one switch here that
+                   changes what a step computes: gradients are taken at the restored rows, and so are the signs of the ReLUs that
+                   the BatchNorm sweeps have folded in.  In 8 bits the layers run one by one (the fused sparse nodes keep full
+                   rows) and TrainStep leaves its step arena aside, so that rows are freed as the forward pass goes on; default
+                   "full"                                                                             [D3D_ACTIVATIONS]
   step_arena       TrainStep's default for its step arena (arena.py)
   geometry_ring    slots of GeometryPrefetcher's arena ring (0 = caching allocator)
 

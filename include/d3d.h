@@ -469,7 +469,8 @@ int d3d_channel_affine_bwd(const void *x, const void *dy, int n, int c, int dtyp
 /* ------------------------------------------------------------------------
  * Rows held in 8 bits between the forward and the backward pass (csrc/d3d_act8.hip).  The reference keeps every activation
  * of a training step in full (autograd's saved tensors behind det3d/models/backbones/scn.py:106-157); a held row takes 33
- * bytes for every 32 channels begun (1.03 a value).  32 consecutive channels of a row form a group with one scale 2^s, stored as the biased exponent s + 127:
+ * bytes for every 32 channels begun (1.03 a value).  32 consecutive channels of a row form a group with one scale 2^s, stored as
+ * the biased exponent s + 127:
  *   D3D_ACT8_INT8  s the smallest with rint(max|x| 2^-s) <= 127, s in [-120, 121]; codes int8 rint(x 2^-s), clipped to +-127
  *   D3D_ACT8_E4M3  s the smallest with max|x| 2^-s <= 448, s in [-110, 119];       codes OCP e4m3 of x 2^-s, clipped to +-448
  * A group with a NaN or an infinity has scale byte 255 and is restored as NaN.  Restored values are exact in bf16.

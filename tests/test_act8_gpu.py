@@ -385,3 +385,24 @@ def test_tables_that_end_with_their_buffer(act8, n, kvol, cin):
     nbr = table(n, n, kvol, 0.5, n)
     nbr[-1] = torch.arange(n, dtype=torch.int32).flip(0)
     check_dw(act8.weight_grad(act8.hold(x, "int8"), dy, nbr.cuda()), restored(x, "int8"), dy, nbr)
+
+
+def test_small_gradients(act8):
+    """dy down to the smallest numbers: the three bfloat16 terms leave at most 2^-134 of a value (half of bfloat16's smallest step),
+    and a sum below the normal numbers is rounded to 2^-149 at every addition"""
+    x = rows(64, 40, torch.float32, 1)
+    g = torch.Generator().manual_seed(5)
+    dy = (1 + torch.rand(64, 24, generator=g)) * torch.exp2(-100 - torch.randint(0, 45, (64, 24), generator=g).float())
+    x64 = restored(x, "int8")
+    got = act8.weight_grad(act8.hold(x), dy.cuda())
+    want, mag = reference_dw(x64, dy, None)
+    tol = 68 * EPS32 * mag + 2.0 ** -134 * x64.abs().sum(0)[:, None] + 3 * 64 * 2.0 ** -149
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+    exact = dy.abs() >= 2.0 ** -110
+    one = torch.zeros(64, 40)
+    one[:, 0] = 1
+    dy1 = torch.where(exact, dy, torch.zeros(()))
+    for r in range(0, 64, 16):  # one row alone: the value itself
+        single = torch.zeros_like(dy1)
+        single[r] = dy1[r]
+        assert torch.equal(act8.weight_grad(act8.hold(one.cuda()), single.cuda())[0].cpu(), single[r])

@@ -536,7 +536,8 @@ static int rj_check(const D3dRowJoin *a, bool backward, const char *who) {
   D3D_REQUIRE(held == (a->x_scales != nullptr) && (a->f_codes != nullptr) == (a->f_scales != nullptr), "%s: codes without scales", who);
   const bool has_f = a->f || a->f_codes;
   D3D_REQUIRE(!backward || !held || !has_f || a->f_codes, "%s: x is held in 8 bits, f is not", who);
-  D3D_REQUIRE(!has_f || (backward && !a->f_codes) || held == (a->f_codes != nullptr) || (!a->pre_kind && a->f_codes), "%s: x and f are held together", who);
+  D3D_REQUIRE(!has_f || (backward && !a->f_codes) || held == (a->f_codes != nullptr) || (!a->pre_kind && a->f_codes),
+              "%s: x and f are held together", who);
   D3D_REQUIRE(backward || a->f || !a->f_codes, "%s: codes of f without f", who);
   D3D_REQUIRE(a->post_kind >= 0 && a->post_kind <= 2 && a->pre_kind >= 0 && a->pre_kind <= 2, "%s: norm kinds %d, %d", who, a->post_kind, a->pre_kind);
   D3D_REQUIRE(a->post_eps >= 0.f && a->pre_eps >= 0.f, "%s: negative eps", who);
